@@ -28,56 +28,49 @@ def _package():
         sys.path.insert(0, pkg)
 
 
-_KEPT = []
-
-
 def _context():
-    """The framework's device context, imported and looked up once, as a
-    program does."""
-    if not _KEPT:
-        _package()
-        from ttrl_b200.device import context
-        _KEPT.append(context("cuda:0"))
-    return _KEPT[0]
+    _package()
+    from ttrl_b200.device import context
+    return context("cuda:0")
 
 
 def listed():
     return [
         # One acting step of a small set of environments: latency.
-        {"name": "attention step 16 lanes", "op": "step", "batch": 16, "heads": 4, "key": 64,
+        {"name": "attention step, 16 lanes", "op": "step", "batch": 16, "heads": 4, "key": 64,
          "value": 64, "starts": True},
         # One acting step of a large vectorised simulator: the state's bytes.
-        {"name": "attention step 4096 lanes", "op": "step", "batch": 4096, "heads": 4,
+        {"name": "attention step, 4096 lanes", "op": "step", "batch": 4096, "heads": 4,
          "key": 64, "value": 64, "starts": True},
         # The recurrent PPO minibatch (16 sequences of 32 steps), with resets.
-        {"name": "attention train 32x16", "op": "attention", "train": True, "steps": 32,
+        {"name": "attention train, 32x16", "op": "attention", "train": True, "steps": 32,
          "batch": 16, "heads": 4, "key": 64, "value": 64, "starts": True},
         # Few long contexts, odd length: the time axis has to be split.
-        {"name": "attention forward 8191x2", "op": "attention", "train": False, "steps": 8191,
+        {"name": "attention forward, 8191x2", "op": "attention", "train": False, "steps": 8191,
          "batch": 2, "heads": 8, "key": 64, "value": 64, "starts": False},
         # Many episodes of a long rollout, unequal key and value widths.
-        {"name": "attention train 1024x64", "op": "attention", "train": True, "steps": 1024,
+        {"name": "attention train, 1024x64", "op": "attention", "train": True, "steps": 1024,
          "batch": 64, "heads": 8, "key": 64, "value": 128, "starts": True},
         # The third conv layer of an acting batch: latency.
-        {"name": "norm forward 32x7x7x64", "op": "norm", "train": False, "images": 32,
+        {"name": "norm forward, 32x7x7x64", "op": "norm", "train": False, "images": 32,
          "spatial": 49, "channels": 64, "groups": 8, "act": "relu"},
         # The first conv layer of a PPO minibatch.
-        {"name": "norm train 256x20x20x32", "op": "norm", "train": True, "images": 256,
+        {"name": "norm train, 256x20x20x32", "op": "norm", "train": True, "images": 256,
          "spatial": 400, "channels": 32, "groups": 4, "act": "silu"},
         # The head norm behind the memory: one row a token.
-        {"name": "norm train 32768x512", "op": "norm", "train": True, "images": 32768,
+        {"name": "norm train, 32768x512", "op": "norm", "train": True, "images": 32768,
          "spatial": 1, "channels": 512, "groups": 8, "act": "silu"},
         # A wide residual stage of a large batch, with groups of odd width.
-        {"name": "norm train 512x42x42x90", "op": "norm", "train": True, "images": 512,
+        {"name": "norm train, 512x42x42x90", "op": "norm", "train": True, "images": 512,
          "spatial": 1764, "channels": 90, "groups": 6, "act": "silu"},
         # The recurrent actor-critic's update.
-        {"name": "adamw recurrent net", "op": "adamw", "sizes": _RECURRENT_NET, "tensors": 16,
+        {"name": "adamw, recurrent net", "op": "adamw", "sizes": _RECURRENT_NET, "tensors": 16,
          "params": 2277287, "bits": 32},
         # A deep net: hundreds of tensors, most of them short.
-        {"name": "adamw 320 tensors", "op": "adamw", "sizes": "", "tensors": 320,
+        {"name": "adamw, 320 tensors", "op": "adamw", "sizes": "", "tensors": 320,
          "params": 24000000, "bits": 32},
         # The largest: states in 8 bits, read back as a checkpoint reads them.
-        {"name": "adamw 8 bits 96 tensors", "op": "adamw", "sizes": "", "tensors": 96,
+        {"name": "adamw, 8 bits, 96 tensors", "op": "adamw", "sizes": "", "tensors": 96,
          "params": 100000000, "bits": 8},
     ]
 
