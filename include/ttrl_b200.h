@@ -710,7 +710,11 @@ size_t ttrl_group_norm_workspace_bytes(int images, int spatial, int channels, in
  * [steps][batch][heads * value_dim]. state (NULL: zero) and new_state (NULL:
  * not written) are [batch][heads][key_dim][value_dim]. starts
  * ([steps][batch], NULL: none): where it is not 0 the state is dropped before
- * the token, whatever it holds. decay: [heads] floats in [0, 1]. key_dim,
+ * the token, whatever it holds. A token's error is a few 2^-22 of the sum of
+ * decay^n |q| |k| |v| that its output is made of (2-norms; in a column of v of
+ * that column), whatever the size of other tokens, episodes and columns (a
+ * chunk whose columns differ by more than about 2^17 is done in fp32, at ten
+ * times its time). decay: [heads] floats in [0, 1]. key_dim,
  * value_dim up to 128. No result may overlap an operand. `workspace` is laid out as the GEMM's (64 KB of
  * counters, left as they are, then scratch). No reference counterpart (its
  * only memory is the GRU, ttrl/engine/recurrent.py:45-168). */

@@ -21,10 +21,17 @@
 // copy in shared memory) along the chunks, so q, k and v are read once and
 // o written once: 4 (2K + 2V) bytes a token and head is the floor.
 //
-// The products must be good to fp32, on tensor cores. Each operand tile gets
-// a power of two that brings its largest value just below 2^15, and each
+// The products must be good to fp32, on tensor cores. Each row of q, k and v
+// gets a power of two that brings its largest value just below 2^15 (the state
+// has one for all of it), and each
 // value is held as two half-precision numbers, hi and x - hi: 22 bits, down to
-// values 2^-18 of the tile's largest, and 2^-40 of that below. A product is
+// values 2^-18 of the row's largest, and 2^-40 of that below. The powers of k's
+// and v's rows go into the weight of their token's scores, and a row of weighted
+// scores, split in its turn, is divided by the largest token that it sees: a
+// token's error goes by what its own result is made of, not by a larger token in
+// the same tile, in an episode that a start has dropped or later in time. (One
+// power a tile took 13% less time, and lost all bits of a token beside one 10^12
+// times its size; done in fp32, a chunk takes ten times as long.) A product is
 // hi hi + hi lo + lo hi, three mma.sync of 16-bit operands at twice the rate
 // that two-part tf32 has. k, v and the state are split once, as they are
 // stored in shared memory, and ldmatrix reads either orientation; a warp's
@@ -39,16 +46,17 @@
 //
 // Times on B200, forward and backward (three scans in one launch, or two where
 // key and value pad differently), shares of the measured copy rate in brackets:
-//   32 tokens x 16 lanes x 4 heads of 64/64: 11 and 14 us: one chunk's chain of
+//   32 tokens x 16 lanes x 4 heads of 64/64: 12 and 15 us: one chunk's chain of
 //     loads, splits and products, mostly first fetches of instructions
-//   512 x 256 x 4 of 32/32: 112 (37%) and 293 us
-//   1024 x 64 x 8 of 64/64: 201 (41%) and 538 us; of 64/128: 363 and 964 us
-//   2048 x 8 x 8 of 128/128: 153 and 457 us
-//   8191 x 2 x 8 of 64/64: 96 and 259 us, in segments
+//   512 x 256 x 4 of 32/32: 121 (34%) and 325 us
+//   1024 x 64 x 8 of 64/64: 234 (36%) and 625 us; of 64/128: 416 and 1148 us
+//   2048 x 8 x 8 of 128/128: 172 and 530 us
+//   8191 x 2 x 8 of 64/64: 115 and 313 us, in segments
 //
 // A product with a masked-out factor multiplies by zero, which infinities and
 // NaN survive. So a chunk whose results are not all finite is done again
-// token by token, from the recurrence itself.
+// token by token in fp32, from the recurrence itself (la_exact); so is one whose
+// columns differ in size by more than the halves hold (kLaShort).
 //
 // Few lanes and heads with many tokens: the scan is cut into segments. One
 // launch gives each segment's state from nothing, a second adds them up in
@@ -138,13 +146,85 @@ __device__ __forceinline__ float tile_scale(uint32_t max_bits) {
   e = max(-40, min(80, e));
   return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
 }
-// Scores of two such tiles are below 128 * 2^30: times this, a half.
-constexpr float kScoreScale = 1.f / (1 << 22);
 // Of a power of two. Products of such inverses may run out of range to zero,
 // as what they scale does; a product of the powers themselves may not.
 __device__ __forceinline__ float pow2_inverse(float s) {
   return __uint_as_float((254u << 23) - __float_as_uint(s));
 }
+
+// A row of k or v has a power of two of its own, that brings its largest value to
+// [2^14, 2^15): from 2^-40 to 2^62. No power (kLaNone) for a row of zeros.
+constexpr int kLaNone = -128, kLaLeast = -40, kLaMost = 62;
+__device__ __forceinline__ int row_exp(uint32_t max_bits) {
+  if (max_bits == 0) return kLaNone;
+  return max(kLaLeast, min(kLaMost, 141 - static_cast<int>(max_bits >> 23)));
+}
+__device__ __forceinline__ float pow2(int e) {  // -126 .. 127
+  return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+__device__ __forceinline__ float row_scale(int e) { return e == kLaNone ? 1.f : pow2(e); }
+// The power of two above x > 0; 1 for 0.
+__device__ __forceinline__ float pow2_above(float x) {
+  return x == 0.f ? 1.f : pow2(max(-126, static_cast<int>(__float_as_uint(x) >> 23) - 126));
+}
+// A token's size, the inverse of what its k and v were scaled by, as the
+// exponent of a float (3 to 207; 0 where either is zero).
+__device__ __forceinline__ uint32_t token_size(int ek, int ev) {
+  return ek == kLaNone || ev == kLaNone ? 0u : static_cast<uint32_t>(127 - ek - ev);
+}
+__device__ __forceinline__ float size_float(uint32_t size) { return __uint_as_float(size << 23); }
+// Tokens alike within 2^8: then the bound of a row's scores is the largest
+// token's, which costs them 2^8 of the 2^32 that their halves hold beside the
+// typical one.
+constexpr uint32_t kLaAlike = 8;
+// The largest of the LANES neighbouring lanes that share a row.
+template <int LANES>
+__device__ __forceinline__ uint32_t row_max(uint32_t x) {
+  if constexpr (LANES == 32) {
+    return __reduce_max_sync(0xffffffffu, x);
+  } else if constexpr (LANES == 16) {
+    const bool low = (threadIdx.x & 16) == 0;
+    const uint32_t a = __reduce_max_sync(0xffffffffu, low ? x : 0u);
+    const uint32_t b = __reduce_max_sync(0xffffffffu, low ? 0u : x);
+    return low ? a : b;
+  } else {
+#pragma unroll
+    for (int o = 1; o < LANES; o *= 2) x = max(x, __shfl_xor_sync(0xffffffffu, x, o));
+    return x;
+  }
+}
+// What the halves cannot hold. A scaled value below 2^-3 (kLaShort) keeps fewer
+// than 22 bits. One by chance (one normal value in 80,000) does not show in its
+// column's norm; columns that differ in size have many, and the small one's
+// results need them. So a chunk is done in fp32, token by token, where la_spare
+// threads have such values in la_rows of their rows (a column is at least four
+// threads'). That q's columns differ does no harm unless k's do too, and that the
+// state's do none where every token of the chunk weighs as much as 2^-18 of
+// the state: then its column is of that size (la_dwarfs).
+constexpr int kLaShort = 127 - 3;  // an exponent as in a float's bits
+// Twice the bits of the smaller magnitude, less one: zero is the largest.
+__device__ __forceinline__ uint32_t least2(float x, float y) {
+  return min(__float_as_uint(x) * 2u - 1u, __float_as_uint(y) * 2u - 1u);
+}
+// Whether one of the magnitudes behind `least`, times 2^e, is short of bits.
+__device__ __forceinline__ int la_short(uint32_t least, int e) {
+  return least < (static_cast<uint32_t>(kLaShort - e) << 24) - 1u;
+}
+__device__ __forceinline__ int la_short(const float (&x)[4], int e) {
+  return la_short(min(least2(x[0], x[1]), least2(x[2], x[3])), e == kLaNone ? 0 : e);
+}
+// Whether a state scaled by 2^es is more than that beside tokens of this least
+// size (0: tokens of zeros).
+__device__ __forceinline__ bool la_dwarfs(int es, uint32_t least_size) {
+  return es + static_cast<int>(least_size) + 30 < 127;
+}
+__device__ __forceinline__ int la_rows(int len) { return len >= 64 ? 2 : 1; }
+__device__ __forceinline__ int la_spare(const LaArgs& a, int len) {
+  return len >= 64 ? 2 : 1 + min(3, (len * (a.kd + a.vd)) >> 11);
+}
+
+// Scores of two such tiles are below 128 * 2^30: times this, a half.
+constexpr float kScoreScale = 1.f / (1 << 22);
 
 __device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0,
                                       uint32_t b1) {
@@ -196,8 +276,9 @@ struct LaTile {
   static constexpr int kV = kLaChunk * kLdV * 2;
   static constexpr int kS = DK * kLdV * 2;
   static constexpr int kK0 = 0, kV0 = 2 * kK, kS0 = kV0 + 2 * kV;
-  static constexpr int kRest = kS0 + 2 * kS;               // pw, wt, cnt, mask, maxima
-  static constexpr int kBytes = kRest + (16 + 3 * kLaChunk + 4 + 2 + 12 + 2) * 4;
+  // pw, wt, cnt, mask, state maxima, the sum's scale; kf, rows, exponents
+  static constexpr int kRest = kS0 + 2 * kS;
+  static constexpr int kBytes = kRest + (16 + 3 * kLaChunk + 4 + 2 + 4 + 2) * 4 + 10 * kLaChunk;
 };
 
 // One tile of `rows` tokens by `cols` floats (the rest zeros) in registers, 4
@@ -224,32 +305,36 @@ __device__ __forceinline__ void load_tile(float (&x)[kLaChunk * D / (4 * kLaThre
     }
   }
 }
-template <int N>
-__device__ __forceinline__ uint32_t tile_max(const float (&x)[N][4]) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int u = 0; u < N; ++u)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = max(m, __float_as_uint(x[u][e]) & 0x7fffffffu);
-  return m;
-}
-// The same slots, scaled and split, into a shared tile.
+// The same slots, each row scaled by its own power of two and split, into a
+// shared tile; the powers' exponents to exps[row]. False where a row is not
+// finite, or too small for the powers there are.
 template <int D>
-__device__ __forceinline__ void store_tile(uint32_t base, uint32_t part,
+__device__ __forceinline__ bool store_tile(uint32_t base, uint32_t part,
                                            const float (&x)[kLaChunk * D / (4 * kLaThreads)][4],
-                                           float scale) {
+                                           int8_t* exps, int& lost) {
   constexpr int Q = D / 4, N = kLaChunk * D / (4 * kLaThreads);
-  const uint32_t at =
-      base + ((threadIdx.x / Q) * (D + 8) + (threadIdx.x % Q) * 4) * 2;
+  const int r0 = threadIdx.x / Q;
+  const uint32_t at = base + (r0 * (D + 8) + (threadIdx.x % Q) * 4) * 2;
+  bool fine = true;
 #pragma unroll
   for (int u = 0; u < N; ++u) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[u][e]) & 0x7fffffffu);
+    top = row_max<Q>(top);
+    const int e = row_exp(top);
+    fine &= top < 0x7f800000u && (top == 0 || (top >> 23) >= 141 - kLaMost);
+    lost += la_short(x[u], e);
+    const float scale = row_scale(e);
+    if (threadIdx.x % Q == 0) exps[r0 + u * (kLaThreads / Q)] = static_cast<int8_t>(e);
     uint32_t h0, h1, l0, l1;
-    split2(x[u][0] * scale, x[u][1] * scale, h0, l0);
-    split2(x[u][2] * scale, x[u][3] * scale, h1, l1);
+    split2(x[u][0], x[u][1], scale, h0, l0);
+    split2(x[u][2], x[u][3], scale, h1, l1);
     const uint32_t to = at + u * (kLaThreads / Q) * (D + 8) * 2;
     asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to), "r"(h0), "r"(h1) : "memory");
     asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + part), "r"(l0), "r"(l1) : "memory");
   }
+  return fine;
 }
 
 // Not zero where a start lies before token `place` of the scan (its own start;
@@ -258,6 +343,56 @@ __device__ __forceinline__ float la_start(const LaArgs& a, int place, int lane) 
   if (a.starts == nullptr || (a.reverse && place == 0)) return 0.f;
   const int token = a.reverse ? a.steps - place : place;
   return a.starts[static_cast<int64_t>(token) * a.batch + lane];
+}
+
+// A chunk of `len` tokens from the recurrence itself, in fp32: the state is in
+// `ss` ([DK][LD]) before and behind it. A thread has one column and DK / (TH /
+// DV) rows of it in registers; the sums over rows meet in `part` (32 tokens of
+// TH floats), so a token costs no barrier. drop(i): a start before token i.
+template <int DK, int DV, int LD, int TH, bool OUT, typename F>
+__device__ __forceinline__ void la_exact(const LaArgs& a, float* ss, float* part, int64_t row,
+                                         int64_t dir, int len, int lead, int h, int v0, int vcols,
+                                         float decay, F&& drop) {
+  constexpr int G = TH / DV, R = DK / G, TOKENS = 32;
+  const int col = threadIdx.x % DV, grp = threadIdx.x / DV, r0 = grp * R;
+  const bool mine = col < vcols;
+  float s[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) s[r] = ss[(r0 + r) * LD + col];
+  for (int i0 = 0; i0 < len; i0 += TOKENS) {
+    const int n = min(TOKENS, len - i0);
+    for (int i = 0; mine && i < n; ++i) {
+      const int64_t at = row + (i0 + i) * dir;
+      const float f = i0 + i == 0 && lead == 0 ? 1.f : decay;
+      const bool gone = drop(i0 + i);
+      const float* k = a.k + at * a.ldk + h * a.kd + r0;
+      const float* q = a.q + at * a.ldq + h * a.kd + r0;
+      const float v = a.v[at * a.ldv + h * a.vd + v0 + col];
+      float sum = 0.f;
+#pragma unroll
+      for (int r = 0; r < R; ++r) {
+        if (r0 + r >= a.kd) continue;
+        s[r] = fmaf(k[r] * a.kscale, v, gone ? 0.f : s[r] * f);
+        if (OUT) sum = fmaf(q[r], s[r], sum);
+      }
+      if (OUT) part[(i * G + grp) * DV + col] = sum;
+    }
+    if (OUT) {
+      __syncthreads();
+      for (int e = threadIdx.x; e < n * DV; e += TH) {
+        const int i = e / DV, c = e % DV;
+        if (c >= vcols) continue;
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < G; ++w) sum += part[(i * G + w) * DV + c];
+        a.o[(row + (i0 + i) * dir) * a.ldo + h * a.vd + v0 + c] = sum * a.scale;
+      }
+      __syncthreads();
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < R; ++r) ss[(r0 + r) * LD + col] = s[r];
+  __syncthreads();
 }
 
 __device__ __forceinline__ void prefetch_l2(const void* p) {
@@ -285,7 +420,11 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
   float* wt = pw + kLaChunk + 4;                         // weight of a token in the state
   int* cnt = reinterpret_cast<int*>(wt + kLaChunk);      // starts up to a token, its own included
   uint32_t* mask = reinterpret_cast<uint32_t*>(cnt + kLaChunk);  // [2]
-  uint32_t* maxima = mask + 2;                                   // [4 warps][k, v, state]
+  uint32_t* maxima = mask + 2;                                   // [4 warps], of the state
+  float* sum_up = reinterpret_cast<float*>(maxima + 4);          // [1] of the state's sum
+  float* kf = sum_up + 2;        // a token's size
+  float* reach = kf + kLaChunk;  // the size of what a row's scores may add up
+  int8_t* kexp = reinterpret_cast<int8_t*>(reach + kLaChunk);  // of k's rows, then v's
   const uint32_t sbase = smem_u32(la_smem);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int g = lane >> 2, c = lane & 3;
@@ -354,10 +493,11 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
     const int len = min(kLaChunk, end - c0);
     const int lead = c0 == 0 && a.reverse ? 0 : 1;
     const int64_t row = static_cast<int64_t>(a.reverse ? a.steps - 1 - c0 : c0) * a.batch + b;
-    float sk, sv, sst = 1.f;  // the tiles' powers of two
+    float sst = 1.f;  // the state's power of two
     uint64_t starts;
     int total;
-    bool finite;
+    bool finite;   // and within what the halves hold
+    int lost = 0;  // rows with values short of bits
     {
       float xk[kLaChunk * DK / (4 * kLaThreads)][4], xv[kLaChunk * DV / (4 * kLaThreads)][4];
       uint32_t flag = 0;
@@ -371,39 +511,98 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
 #pragma unroll
           for (int e = 0; e < 4; ++e) xk[u][e] *= a.kscale;
       }
-      uint32_t top[3] = {tile_max(xk), tile_max(xv), 0};
-      if (OUT)
+      finite = store_tile<DK>(sbase + T::kK0, T::kK, xk, kexp, lost);
+      finite &= store_tile<DV>(sbase + T::kV0, T::kV, xv, kexp + kLaChunk, lost);
+      if (OUT) {
+        uint32_t top = 0;
         each_state([&](float& held, int, int) {
-          top[2] = max(top[2], __float_as_uint(held) & 0x7fffffffu);
+          top = max(top, __float_as_uint(held) & 0x7fffffffu);
         });
-#pragma unroll
-      for (int i = 0; i < (OUT ? 3 : 2); ++i) {
-        top[i] = __reduce_max_sync(0xffffffffu, top[i]);
-        if (lane == 0) maxima[warp * 3 + i] = top[i];
+        top = __reduce_max_sync(0xffffffffu, top);
+        if (lane == 0) maxima[warp] = top;
       }
       if (warp < 2 && lane == 0) mask[warp] = flag;
-      __syncthreads();  // and every warp is done with the last chunk's tiles
+    }
+    __syncthreads();
+    starts = mask[0] | static_cast<uint64_t>(mask[1]) << 32;
+    total = __popcll(starts);
+    uint32_t low = 255;  // the least of the tokens' sizes
+    {
+      uint32_t size[2], high = 0;
+      bool zeros = false;
 #pragma unroll
-      for (int i = 0; i < (OUT ? 3 : 2); ++i)
-        top[i] = max(max(maxima[i], maxima[3 + i]), max(maxima[6 + i], maxima[9 + i]));
-      starts = mask[0] | static_cast<uint64_t>(mask[1]) << 32;
-      total = __popcll(starts);
-      if (tid < kLaChunk) {
-        const int n = __popcll(starts & (~0ull >> (63 - tid)));
-        cnt[tid] = n;
-        wt[tid] = tid < len && n == total ? pw[len - 1 - tid] * (1.f / kScoreScale) : 0.f;
+      for (int w = 0; w < 2; ++w) {
+        const int j = w * 32 + lane;
+        size[w] = token_size(kexp[j], kexp[kLaChunk + j]);
+        high = max(high, size[w]);
+        low = min(low, size[w] == 0 ? 255u : size[w]);
+        zeros |= size[w] == 0 && j < len;
       }
-      finite = max(max(top[0], top[1]), top[2]) < 0x7f800000u;
-      sk = tile_scale(top[0]);
-      sv = tile_scale(top[1]);
-      store_tile<DK>(sbase + T::kK0, T::kK, xk, sk);
-      store_tile<DV>(sbase + T::kV0, T::kV, xv, sv);
+      high = __reduce_max_sync(0xffffffffu, high);
+      low = __reduce_min_sync(0xffffffffu, zeros ? 0u : low);
+      if (tid < kLaChunk) {
+        const uint64_t upto = starts & (~0ull >> (63 - tid));
+        const float f[2] = {size_float(size[0]), size_float(size[1])};
+        const float mine = warp == 0 ? f[0] : f[1];
+        const int last = starts == 0 ? 0 : 63 - __clzll(starts);
+        const float w = tid >= last && tid < len ? mine * (pw[len - 1 - tid] * (1.f / kScoreScale))
+                                                 : 0.f;
+        float m = size_float(high), most = m;
+        if (high > low + kLaAlike) {
+          // The state's sum: against the largest token at its weight.
+          const int other = tid ^ 32;
+          const float w2 = other >= last && other < len
+                               ? (warp == 0 ? f[1] : f[0]) * (pw[len - 1 - other] * (1.f / kScoreScale))
+                               : 0.f;
+          most = __uint_as_float(
+              __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(w, w2))));
+          // The largest token that a row sees, at its weight: of the rows before
+          // it in the warp, then of the first half.
+          const int own = upto == 0 ? -1 : 63 - __clzll(upto);
+          m = mine;
+#pragma unroll
+          for (int o = 1; o < 32; o *= 2) {
+            const float before = __shfl_up_sync(0xffffffffu, m, o);
+            if (lane >= o && tid - o >= own)
+              m = fmaxf(m, before * (pw[o] * (1.f / kScoreScale)));
+          }
+          if (warp == 1) {
+            const uint32_t early = static_cast<uint32_t>(starts);
+            const int from = early == 0 ? -1 : 31 - __clz(early);
+            const float carry = __uint_as_float(__reduce_max_sync(
+                0xffffffffu, __float_as_uint(lane >= from ? f[0] * (pw[32 - lane] *
+                                                                    (1.f / kScoreScale))
+                                                          : 0.f)));
+            if (own < 32) m = fmaxf(m, carry * (pw[lane] * (1.f / kScoreScale)));
+          }
+        }
+        const float up = pow2_above(most);
+        cnt[tid] = __popcll(upto);
+        kf[tid] = mine;
+        wt[tid] = w * pow2_inverse(up);
+        reach[tid] = pow2_above(m);
+        if (tid == 0) *sum_up = up;
+      }
       if constexpr (OUT) {
-        sst = tile_scale(top[2]);
+        const uint32_t top = max(max(maxima[0], maxima[1]), max(maxima[2], maxima[3]));
+        finite &= top < 0x7f800000u;
+        sst = tile_scale(top);
+        const int es = static_cast<int>(__float_as_uint(sst) >> 23) - 127;
+        if (la_dwarfs(es, low)) {
+          int few = 0;
+#pragma unroll
+          for (int m = 0; m < MT; ++m)
+#pragma unroll
+            for (int n = 0; n < NS; ++n) {
+              few += la_short(least2(st[m][n][0], st[m][n][1]), es);
+              few += la_short(least2(st[m][n][2], st[m][n][3]), es);
+            }
+          if (few >= (a.kd > 8 && vcols > 8 ? 2 : 1)) finite = false;
+        }
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
-          for (int n = 0; n < NS; ++n)
+          for (int n = 0; n < NS; ++n) {
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               uint32_t hi, lo;
@@ -413,6 +612,7 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
               *reinterpret_cast<uint32_t*>(to) = hi;
               *reinterpret_cast<uint32_t*>(to + T::kS) = lo;
             }
+          }
       }
     }
     any_start |= total;
@@ -435,11 +635,10 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
     // at no harm but time, if it overflows).
     float check = 0.f;
     const float keep = total == 0 ? pw[len - 1 + lead] * (1.f / kScoreScale) : 0.f;
-
     if constexpr (OUT) {
-      // This warp's rows of q, split at their own scale.
+      // This warp's rows of q, split at their own scales.
       Frag q[NK];
-      float sq;
+      float sq[2];
       {
         float x[NK][8];
         const int r0 = rb + g, r1 = rb + g + 8;
@@ -463,20 +662,25 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
             x[k][half * 4] = t0.x, x[k][half * 4 + 1] = t0.y;
             x[k][half * 4 + 2] = t1.x, x[k][half * 4 + 3] = t1.y;
           }
-        __syncthreads();
-        uint32_t top = 0;
 #pragma unroll
-        for (int k = 0; k < NK; ++k)
+        for (int half = 0; half < 2; ++half) {
+          uint32_t top = 0;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) top = max(top, __float_as_uint(x[k][e]) & 0x7fffffffu);
-        top = __reduce_max_sync(0xffffffffu, top);
-        finite &= top < 0x7f800000u;
-        sq = tile_scale(top);
+          for (int k = 0; k < NK; ++k)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              top = max(top, __float_as_uint(x[k][(e >> 1) * 4 + half * 2 + (e & 1)]) & 0x7fffffffu);
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+          sq[half] = tile_scale(top);
+          finite &= top < 0x7f800000u;
+        }
+        finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(a, len);
 #pragma unroll
         for (int k = 0; k < NK; ++k)
 #pragma unroll
           for (int i = 0; i < 4; ++i)
-            split2(x[k][2 * i] * sq, x[k][2 * i + 1] * sq, q[k].hi[i], q[k].lo[i]);
+            split2(x[k][2 * i] * sq[i & 1], x[k][2 * i + 1] * sq[i & 1], q[k].hi[i], q[k].lo[i]);
       }
       // c_i q_i S, then brought to the scale of the scores' product with v.
       float o[NV][4];
@@ -493,10 +697,12 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
           mma3(o[n], o[n + 1], q[k], s);
         }
       const int n0 = cnt[rb + g], n1 = cnt[rb + g + 8];
+      // A row's scores are divided by `reach`.
+      const float down0 = reach[rb + g], down1 = reach[rb + g + 8];
+      const float up0 = pow2_inverse(down0), up1 = pow2_inverse(down1);
       {
-        const float up = sk * pow2_inverse(sst) * sv;
-        const float e0 = n0 == 0 ? pw[rb + g + lead] * up : 0.f;
-        const float e1 = n1 == 0 ? pw[rb + g + 8 + lead] * up : 0.f;
+        const float e0 = n0 == 0 ? pw[rb + g + lead] * (pow2_inverse(sst) * up0) : 0.f;
+        const float e1 = n1 == 0 ? pw[rb + g + 8 + lead] * (pow2_inverse(sst) * up1) : 0.f;
 #pragma unroll
         for (int n = 0; n < NV; ++n)
 #pragma unroll
@@ -530,10 +736,11 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
           const float* t = pi - j0 - n * 8;
-          p[n][0] = (p[n][0] + (p1[n][0] + p2[n][0])) * t[0];
-          p[n][1] = (p[n][1] + (p1[n][1] + p2[n][1])) * t[-1];
-          p[n][2] = (p[n][2] + (p1[n][2] + p2[n][2])) * t[8];
-          p[n][3] = (p[n][3] + (p1[n][3] + p2[n][3])) * t[7];
+          const float2 f = *reinterpret_cast<const float2*>(kf + j0 + n * 8 + 2 * c);
+          p[n][0] = (p[n][0] + (p1[n][0] + p2[n][0])) * t[0] * f.x;
+          p[n][1] = (p[n][1] + (p1[n][1] + p2[n][1])) * t[-1] * f.y;
+          p[n][2] = (p[n][2] + (p1[n][2] + p2[n][2])) * t[8] * f.x;
+          p[n][3] = (p[n][3] + (p1[n][3] + p2[n][3])) * t[7] * f.y;
         }
         if (total != 0) {
 #pragma unroll
@@ -546,10 +753,10 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
           }
         }
         Frag f;
-        split2(p[0][0], p[0][1], f.hi[0], f.lo[0]);
-        split2(p[0][2], p[0][3], f.hi[1], f.lo[1]);
-        split2(p[1][0], p[1][1], f.hi[2], f.lo[2]);
-        split2(p[1][2], p[1][3], f.hi[3], f.lo[3]);
+        split2(p[0][0], p[0][1], up0, f.hi[0], f.lo[0]);
+        split2(p[0][2], p[0][3], up1, f.hi[1], f.lo[1]);
+        split2(p[1][0], p[1][1], up0, f.hi[2], f.lo[2]);
+        split2(p[1][2], p[1][3], up1, f.hi[3], f.lo[3]);
 #pragma unroll
         for (int n = 0; n < NV; n += 2) {
           Frag v;
@@ -557,13 +764,16 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
           mma3(o[n], o[n + 1], f, v);
         }
       }
-      const float down = a.scale * (1.f / kScoreScale) * pow2_inverse(sq) *
-                         pow2_inverse(sk) * pow2_inverse(sv);
+      // In two steps: the inverses' product alone may be too small for float
+      // where the sums that it scales are not.
+      const float down_kv[2] = {down0, down1};
+      const float down_q[2] = {a.scale * (1.f / kScoreScale) * pow2_inverse(sq[0]),
+                               a.scale * (1.f / kScoreScale) * pow2_inverse(sq[1])};
 #pragma unroll
       for (int n = 0; n < NV; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          o[n][e] *= down;
+          o[n][e] = o[n][e] * down_kv[e >> 1] * down_q[e >> 1];
           check += o[n][e];
         }
       // Stored before it is known whether the chunk has to be done again.
@@ -585,12 +795,12 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
         }
       }
     } else {
-      __syncthreads();
+      finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(a, len);
     }
     // The state behind the chunk: this chunk's sum on its own, then one fp32
     // multiply and add.
     float nx[MT][NS][4];
-    const float down = pow2_inverse(sk) * pow2_inverse(sv);
+    const float down = *sum_up;
 #pragma unroll
     for (int m = 0; m < MT; ++m) {
 #pragma unroll
@@ -628,28 +838,12 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
     finite &= isfinite(check);
     if (__syncthreads_or(!finite)) {
       // Token by token, with the state entering the chunk in shared memory in
-      // fp32 (over its halves) and the operands as they are; a thread owns
-      // columns.
+      // fp32 (over its halves) and the operands as they are.
       each_state([&](float& held, int r, int col) { ss[r * LV + col] = held; });
       __syncthreads();
-      for (int i = 0; i < len; ++i) {
-        const bool drop = starts >> i & 1;
-        const float f = i == 0 && lead == 0 ? 1.f : decay;
-        const float* k = a.k + (row + i * dir) * a.ldk + h * a.kd;
-        const float* q = a.q + (row + i * dir) * a.ldq + h * a.kd;
-        for (int col = tid; col < vcols; col += kLaThreads) {
-          float sum = 0.f;
-          const float v = a.v[(row + i * dir) * a.ldv + h * a.vd + v0 + col];
-          for (int r = 0; r < a.kd; ++r) {
-            float s = drop ? 0.f : ss[r * LV + col] * f;
-            s = fmaf(k[r] * a.kscale, v, s);
-            ss[r * LV + col] = s;
-            if (OUT) sum = fmaf(q[r], s, sum);
-          }
-          if (OUT) a.o[(row + i * dir) * a.ldo + h * a.vd + v0 + col] = sum * a.scale;
-        }
-      }
-      __syncthreads();
+      la_exact<DK, DV, LV, kLaThreads, OUT>(a, ss, reinterpret_cast<float*>(la_smem), row, dir,
+                                            len, lead, h, v0, vcols, decay,
+                                            [&](int i) { return starts >> i & 1; });
       each_state([&](float& held, int r, int col) { held = ss[r * LV + col]; });
       continue;
     }
@@ -713,13 +907,20 @@ struct LaTc {
   static constexpr int kS = DK * 64 * 2;
   static constexpr int kBlock = kTcChunk * 128;  // 64 columns of q or k
   static constexpr int kQ0 = 0, kK0 = 2 * kQ, kV0 = 4 * kQ, kS0 = kV0 + 2 * kV;
-  static constexpr int kPw = kS0 + 2 * kS;       // 32 zeros, then d^0 .. d^128
-  static constexpr int kMax = kPw + 164 * 4;     // [k, v, state][warps]
-  static constexpr int kMask = kMax + 3 * kWarps * 4;  // [4]
+  static constexpr int kPw = kS0 + 2 * kS;       // d^0 .. d^128
+  static constexpr int kMax = kPw + 528;         // [warps], of the state
+  static constexpr int kMask = kMax + kWarps * 4;      // [4]
   static constexpr int kExp = kMask + 4 * 4;     // [128] exponents of q's rows
-  static constexpr int kBar = kExp + kTcChunk;   // four
+  // [128] tokens' sizes; where a thread's rows of k are not its rows of v, the
+  // exponents that they come from.
+  static constexpr bool kTwo = DK != 64;
+  static constexpr int kSize = kExp + kTcChunk;
+  static constexpr int kRows = kSize + kTcChunk;  // [k, v][128]
+  static constexpr int kBar = kRows + (kTwo ? 2 * kTcChunk : 0);  // four
   static constexpr int kSlot = kBar + 32;
   static constexpr int kBytes = kSlot + 8;
+  // With what the hardware keeps of each block: two blocks an SM, or one.
+  static_assert((kBytes + 1024) * (DK == 64 ? 2 : 1) <= 228 * 1024, "shared memory");
 };
 // TMEM columns: scores (then their halves, hi and lo in turns of 16 columns),
 // q S (then the chunk's sum for the state), scores v.
@@ -830,15 +1031,10 @@ __device__ __forceinline__ void tc_put(uint32_t to, uint32_t part, const float (
   asm volatile("st.shared.v2.b32 [%0], {%1, %2};" ::"r"(to + part), "r"(l0), "r"(l1) : "memory");
 }
 
-// The largest magnitude, as bits. NaN is passed over: it reaches the results.
-template <int N>
-__device__ __forceinline__ uint32_t tc_max(const float (&x)[N][4]) {
-  float m = 0.f;
-#pragma unroll
-  for (int u = 0; u < N; ++u)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(x[u][e]));
-  return __float_as_uint(m);
+// The largest magnitude of four, as bits. NaN is passed over: it reaches the
+// results.
+__device__ __forceinline__ uint32_t tc_max(const float (&x)[4]) {
+  return __float_as_uint(fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3]))));
 }
 
 template <int DK, int N>
@@ -852,10 +1048,14 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
   constexpr int NV = kTcChunk * 64 / (4 * TH), RV = TH / 16;
   extern __shared__ __align__(1024) uint8_t tc_smem[];
   float* ss = reinterpret_cast<float*>(tc_smem + T::kS0);  // the state in fp32, token by token
-  float* pw = reinterpret_cast<float*>(tc_smem + T::kPw) + 32;  // kScoreScale d^n
+  const float* pw = reinterpret_cast<const float*>(tc_smem + T::kPw);  // kScoreScale d^n
   uint32_t* maxima = reinterpret_cast<uint32_t*>(tc_smem + T::kMax);
   uint32_t* mask = reinterpret_cast<uint32_t*>(tc_smem + T::kMask);
   int8_t* qexp = reinterpret_cast<int8_t*>(tc_smem + T::kExp);
+  int8_t* kexp = reinterpret_cast<int8_t*>(tc_smem + T::kRows);
+  uint8_t* size = tc_smem + T::kSize;
+  // What a row's scores may add up to; over the state, when its product is done.
+  float* reach = reinterpret_cast<float*>(tc_smem + T::kS0);
   const uint32_t sbase = smem_u32(tc_smem);
   const uint32_t bar = sbase + T::kBar;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -884,8 +1084,8 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
   pdl_trigger();
   pdl_wait();
   const float decay = a.decay[h];
-  if (tid < 32 + kTcChunk + 1)
-    pw[tid - 32] = tid < 32 ? 0.f : decay_pow(log2f(decay), tid - 32) * kScoreScale;
+  if (tid <= kTcChunk)
+    reinterpret_cast<float*>(tc_smem + T::kPw)[tid] = decay_pow(log2f(decay), tid) * kScoreScale;
 
   float st[MS][NC][4];
   const int64_t mat = static_cast<int64_t>(bh) * a.kd * a.vd;
@@ -928,69 +1128,89 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
     const int lead = c0 == 0 && a.reverse ? 0 : 1;
     const int64_t row = static_cast<int64_t>(a.reverse ? a.steps - 1 - c0 : c0) * a.batch + b;
     float xv[NV][4];
-    float sk, sv, sst;
+    float sst;
+    bool finite = true;  // and within what the halves hold
+    int lost = 0;        // rows with values short of bits
     {
       float xk[NK][4];
       tc_load<DK, TH>(xk, a.k + h * a.kd, a.ldk, len, a.kd, row, dir, a.vk);
       tc_load<64, TH>(xv, a.v + h * a.vd + v0, a.ldv, len, vcols, row, dir, a.vv);
-      if (a.kscale != 1.f) {
-#pragma unroll
-        for (int u = 0; u < NK; ++u)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) xk[u][e] *= a.kscale;
-      }
       const uint32_t flag = __ballot_sync(0xffffffffu, start != 0.f);
+      if (warp < 4 && lane == 0) mask[warp] = flag;
       float most = 0.f;
       each_state([&](float& held, int, int) { most = fmaxf(most, fabsf(held)); });
-      uint32_t top[3] = {tc_max(xk), tc_max(xv), __float_as_uint(most)};
+      const uint32_t top_s = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+      if (lane == 0) maxima[warp] = top_s;
+      int ek[NK];
 #pragma unroll
-      for (int i = 0; i < 3; ++i) {
-        top[i] = __reduce_max_sync(0xffffffffu, top[i]);
-        if (lane == 0) maxima[i * T::kWarps + warp] = top[i];
+      for (int u = 0; u < NK; ++u) {
+        if (a.kscale != 1.f)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) xk[u][e] *= a.kscale;
+        const uint32_t top = row_max<DK / 4>(tc_max(xk[u]));
+        ek[u] = row_exp(top);
+        finite &= top == 0 || (top >> 23) >= 141 - kLaMost;
+        lost += la_short(xk[u], ek[u]);
+        tc_put(sbase + T::kK0 + tc_slot<DK>() + u * RK * 128, T::kQ, xk[u], row_scale(ek[u]));
+        if (T::kTwo && tid % (DK / 4) == 0)
+          kexp[tid / (DK / 4) + u * RK] = static_cast<int8_t>(ek[u]);
       }
-      if (warp < 4 && lane == 0) mask[warp] = flag;
-      __syncthreads();  // and every thread is done with the last chunk
 #pragma unroll
-      for (int i = 0; i < 3; ++i)
+      for (int u = 0; u < NV; ++u) {
+        const uint32_t top = row_max<16>(tc_max(xv[u]));
+        const int ev = row_exp(top);
+        finite &= top == 0 || (top >> 23) >= 141 - kLaMost;
+        lost += la_short(xv[u], ev);
+        const float scale = row_scale(ev);
 #pragma unroll
-        for (int w = 0; w < T::kWarps; w += 4) {
-          const uint4 x = *reinterpret_cast<const uint4*>(maxima + i * T::kWarps + w);
-          top[i] = max(max(top[i], max(x.x, x.y)), max(x.z, x.w));
+        for (int e = 0; e < 4; ++e) xv[u][e] *= scale;  // and so they stay
+        tc_put(sbase + T::kV0 + tc_slot<64>() + u * RV * 128, T::kV, xv[u], 1.f);
+        if (tid % 16 == 0) {
+          const int r = tid / 16 + u * RV;
+          if (T::kTwo)
+            kexp[kTcChunk + r] = static_cast<int8_t>(ev);
+          else
+            size[r] = static_cast<uint8_t>(token_size(ek[u % NK], ev));
         }
-      sk = tile_scale(top[0]);
-      sv = tile_scale(top[1]);
-      sst = tile_scale(top[2]);
-#pragma unroll
-      for (int u = 0; u < NK; ++u)
-        tc_put(sbase + T::kK0 + tc_slot<DK>() + u * RK * 128, T::kQ, xk[u], sk);
+      }
     }
+    __syncthreads();
+    {
+      uint32_t top = 0;
 #pragma unroll
-    for (int u = 0; u < NV; ++u)
-      tc_put(sbase + T::kV0 + tc_slot<64>() + u * RV * 128, T::kV, xv[u], sv);
+      for (int w = 0; w < T::kWarps; w += 4) {
+        const uint4 x = *reinterpret_cast<const uint4*>(maxima + w);
+        top = max(top, max(max(x.x, x.y), max(x.z, x.w)));
+      }
+      sst = tile_scale(top);
+    }
+    if (T::kTwo && tid < kTcChunk)
+      size[tid] = static_cast<uint8_t>(token_size(kexp[tid], kexp[kTcChunk + tid]));
+    {
 #pragma unroll
-    for (int m = 0; m < MS; ++m)
+      for (int m = 0; m < MS; ++m)
 #pragma unroll
-      for (int n = 0; n < NC; ++n)
+        for (int n = 0; n < NC; ++n) {
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          uint32_t hi, lo;
-          split2(st[m][n][i * 2], st[m][n][i * 2 + 1], sst, hi, lo);
-          const int r = (quarter * MS + m) * 16 + g + i * 8;
-          uint8_t* to = tc_smem + T::kS0 + r * 128 + (((part * NC + n) ^ (r & 7)) << 4) + c * 4;
-          *reinterpret_cast<uint32_t*>(to) = hi;
-          *reinterpret_cast<uint32_t*>(to + T::kS) = lo;
+          for (int i = 0; i < 2; ++i) {
+            uint32_t hi, lo;
+            split2(st[m][n][i * 2], st[m][n][i * 2 + 1], sst, hi, lo);
+            const int r = (quarter * MS + m) * 16 + g + i * 8;
+            uint8_t* to = tc_smem + T::kS0 + r * 128 + (((part * NC + n) ^ (r & 7)) << 4) + c * 4;
+            *reinterpret_cast<uint32_t*>(to) = hi;
+            *reinterpret_cast<uint32_t*>(to + T::kS) = lo;
+          }
         }
+    }
     const uint32_t starts[4] = {mask[0], mask[1], mask[2], mask[3]};
     {
       float xq[NK][4];
       tc_load<DK, TH>(xq, a.q + h * a.kd, a.ldq, len, a.kd, row, dir, a.vq);
-      // A power of two for each slot: one row of 128 columns, two of 64.
+      // A power of two for each row: a slot of a warp is one of 128 columns,
+      // two of 64.
 #pragma unroll
       for (int u = 0; u < NK; ++u) {
-        const uint32_t top = __reduce_max_sync(
-            0xffffffffu, __float_as_uint(fmaxf(fmaxf(fabsf(xq[u][0]), fabsf(xq[u][1])),
-                                               fmaxf(fabsf(xq[u][2]), fabsf(xq[u][3])))));
-        const float sq = tile_scale(top);
+        const float sq = tile_scale(row_max<DK / 4>(tc_max(xq[u])));
         if (tid % (DK / 4) == 0)
           qexp[tid / (DK / 4) + u * RK] =
               static_cast<int8_t>(static_cast<int>(__float_as_uint(sq) >> 23) - 127);
@@ -999,7 +1219,7 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
     }
     fence_proxy_async_smem();
     tc_fence_before();
-    __syncthreads();
+    finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(a, len);
     if (tid == 0 && !dead) {
       tc_fence_after();
       const uint64_t qd = umma_desc(sbase + T::kQ0, 16, 1024, kLayoutSw128);
@@ -1057,10 +1277,68 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
       last = at_high + 31 - __clz(high);
       if (seen != 0) own = at_seen + 31 - __clz(seen);
     }
+    // While the products run: the largest token that this row sees, at its weight,
+    // and the state's sum.
+    float m, most;
+    {
+      uint32_t high = 0, low = 255;
+      bool zeros = false;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t own_size = size[w * 32 + lane];
+        high = max(high, own_size);
+        low = min(low, own_size == 0 ? 255u : own_size);
+        zeros |= own_size == 0 && w * 32 + lane < len;
+      }
+      high = __reduce_max_sync(0xffffffffu, high);
+      low = __reduce_min_sync(0xffffffffu, zeros ? 0u : low);
+      const int es = static_cast<int>(__float_as_uint(sst) >> 23) - 127;
+      if (la_dwarfs(es, low)) {
+        int few = 0;
+#pragma unroll
+        for (int i = 0; i < MS; ++i)
+#pragma unroll
+          for (int n = 0; n < NC; ++n) {
+            few += la_short(least2(st[i][n][0], st[i][n][1]), es);
+            few += la_short(least2(st[i][n][2], st[i][n][3]), es);
+          }
+        if (few >= (a.kd > 8 && vcols > 8 ? 2 : 1)) finite = false;
+      }
+      m = most = size_float(high);
+      if (high > low + kLaAlike) {
+        most = 0.f;
+        float carry = 0.f;
+        int from = -1;  // the last start before this quarter
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+          if (w < quarter && starts[w] != 0) from = w * 32 + 31 - __clz(starts[w]);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const int j = w * 32 + lane;
+          const float f = size_float(size[j]);
+          if (w == quarter) m = f;
+          if (w < quarter && j >= from)
+            carry = fmaxf(carry, f * (pw[quarter * 32 - j] * (1.f / kScoreScale)));
+          if (j >= last && j < len) most = fmaxf(most, f * (pw[len - 1 - j] * (1.f / kScoreScale)));
+        }
+        carry = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(carry)));
+        most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(most)));
+        const int own_row = quarter * 32 + lane;
+#pragma unroll
+        for (int o = 1; o < 32; o *= 2) {
+          const float before = __shfl_up_sync(0xffffffffu, m, o);
+          if (lane >= o && own_row - o >= own)
+            m = fmaxf(m, before * (pw[o] * (1.f / kScoreScale)));
+        }
+        if (own < quarter * 32) m = fmaxf(m, carry * (pw[lane] * (1.f / kScoreScale)));
+      }
+    }
+    const float down_row = pow2_above(m), up_row = pow2_inverse(down_row);
+    const float down_sum = pow2_above(most);
     if (!dead && !mbar_wait(bar, phase)) dead = true;
     tc_fence_after();
-    // w_ij (q_i . k_j) in blocks of 32 tokens; none for later tokens (the
-    // table is zero before d^0).
+    // w_ij (q_i . k_j) in blocks of 32 tokens, at the tokens' sizes, of what the
+    // row may add up to.
 #pragma unroll 1
     for (int j = part; j < 4; j += T::kParts) {
       uint32_t x[32];
@@ -1071,16 +1349,32 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
         uint32_t y[32];
         tmem_ld_row(y, my_rows + kTcP + j * 32);
         const float* t = pw + (quarter - j) * 32 + lane;
+        const uint4* sizes = reinterpret_cast<const uint4*>(size + j * 32);
 #pragma unroll
-        for (int e = 0; e < 32; ++e) y[e] = __float_as_uint(__uint_as_float(y[e]) * t[-e]);
-        if (own > j * 32) {  // none from before the row's own start
-          const uint32_t seen = own < j * 32 + 32 ? 0xffffffffu << (own - j * 32) : 0u;
+        for (int q = 0; q < 2; ++q) {
+          const uint4 four = sizes[q];
+          const uint32_t word[4] = {four.x, four.y, four.z, four.w};
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            const int at = q * 16 + e;
+            const uint32_t w = word[e >> 2];
+            // Byte e & 3 as the exponent of a float.
+            const uint32_t f = (e & 3) == 3 ? w >> 1 : w << (23 - 8 * (e & 3));
+            y[at] = __float_as_uint(__uint_as_float(y[at]) * t[-at] *
+                                    __uint_as_float(f & 0x7f800000u));
+          }
+        }
+        // None from before the row's own start, none behind it.
+        if (own > j * 32 || j == quarter) {
+          uint32_t seen = j == quarter ? 0xffffffffu >> (31 - lane) : 0xffffffffu;
+          if (own > j * 32) seen &= own < j * 32 + 32 ? 0xffffffffu << (own - j * 32) : 0u;
 #pragma unroll
           for (int e = 0; e < 32; ++e) y[e] = seen >> e & 1 ? y[e] : 0;
         }
 #pragma unroll
         for (int e = 0; e < 16; ++e)
-          split2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1]), x[e], x[16 + e]);
+          split2(__uint_as_float(y[2 * e]), __uint_as_float(y[2 * e + 1]), up_row, x[e],
+                 x[16 + e]);
       }
       tmem_st_row(my_rows + kTcP + j * 32, x);
     }
@@ -1095,9 +1389,13 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
 #pragma unroll
     for (int u = 0; u < NV; ++u) {
       const int r = tid / 16 + u * RV;
-      const float w = r >= last ? pw[max(len - 1 - r, 0)] * (1.f / kScoreScale) : 0.f;
-      tc_put(sbase + T::kQ0 + tc_slot<64>() + u * RV * 128, T::kV, xv[u], sv * w);
+      const float w =
+          r >= last ? pw[max(len - 1 - r, 0)] * (1.f / kScoreScale) *
+                          size_float(size[r]) * pow2_inverse(down_sum)
+                    : 0.f;
+      tc_put(sbase + T::kQ0 + tc_slot<64>() + u * RV * 128, T::kV, xv[u], w);
     }
+    if (part == 0) reach[quarter * 32 + lane] = down_row;
     fence_proxy_async_smem();
     tc_fence_before();
     dead = __syncthreads_or(dead);
@@ -1139,15 +1437,17 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
         const int r = quarter * 32 + m * 16 + i * 8 + g;
         const float un = __uint_as_float(static_cast<uint32_t>(127 - qexp[r]) << 23) * a.scale *
                          (1.f / kScoreScale);
-        const float e1 = r < first ? un * pw[r + lead] * pow2_inverse(sst) : 0.f;
-        const float e2 = un * pow2_inverse(sk) * pow2_inverse(sv);
+        // In two steps: a product of the inverses alone may be too small for
+        // float where what they scale is not.
+        const float e1 = r < first ? pw[r + lead] * pow2_inverse(sst) : 0.f;
+        const float e2 = reach[r];
         float* to = a.o + (row + r * dir) * a.ldo + h * a.vd + v0;
 #pragma unroll
         for (int n = 0; n < NC; ++n) {
-          const float x0 = fmaf(e1, __uint_as_float(o1[m][n * 4 + i * 2]),
-                                e2 * __uint_as_float(o2[n * 4 + i * 2]));
-          const float x1 = fmaf(e1, __uint_as_float(o1[m][n * 4 + i * 2 + 1]),
-                                e2 * __uint_as_float(o2[n * 4 + i * 2 + 1]));
+          const float x0 = un * fmaf(e1, __uint_as_float(o1[m][n * 4 + i * 2]),
+                                     e2 * __uint_as_float(o2[n * 4 + i * 2]));
+          const float x1 = un * fmaf(e1, __uint_as_float(o1[m][n * 4 + i * 2 + 1]),
+                                     e2 * __uint_as_float(o2[n * 4 + i * 2 + 1]));
           check += x0 + x1;
           // Stored before it is known whether the chunk has to be done again.
           const int col = part * COLS + n * 8 + 2 * c;
@@ -1165,7 +1465,7 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
     if (!dead) phase ^= 1;
     tc_fence_after();
     const float keep = any == 0 ? pw[len - 1 + lead] * (1.f / kScoreScale) : 0.f;
-    const float down = pow2_inverse(sk) * pow2_inverse(sv);
+    const float down = down_sum;
     float nx[MS][NC][4];
 #pragma unroll
     for (int m = 0; m < MS; ++m) {
@@ -1179,32 +1479,17 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
           check += nx[m][n][e];
         }
     }
-    const bool finite = isfinite(check);
+    finite &= static_cast<bool>(isfinite(check));
     tc_fence_before();
     if (__syncthreads_or(!finite || dead)) {
       dead = __syncthreads_or(dead);
       // Token by token, with the state entering the chunk in shared memory in
-      // fp32 (over its halves) and the operands as they are; a thread owns a
-      // column.
+      // fp32 (over its halves) and the operands as they are.
       each_state([&](float& held, int r, int col) { ss[r * 64 + col] = held; });
       __syncthreads();
-      if (tid < vcols) {
-        for (int i = 0; i < len; ++i) {
-          const bool drop = mask[i >> 5] >> (i & 31) & 1;
-          const float f = i == 0 && lead == 0 ? 1.f : decay;
-          const float* k = a.k + (row + i * dir) * a.ldk + h * a.kd;
-          const float* q = a.q + (row + i * dir) * a.ldq + h * a.kd;
-          const float v = a.v[(row + i * dir) * a.ldv + h * a.vd + v0 + tid];
-          float sum = 0.f;
-          for (int r = 0; r < a.kd; ++r) {
-            const float s = fmaf(k[r] * a.kscale, v, drop ? 0.f : ss[r * 64 + tid] * f);
-            ss[r * 64 + tid] = s;
-            sum = fmaf(q[r], s, sum);
-          }
-          a.o[(row + i * dir) * a.ldo + h * a.vd + v0 + tid] = sum * a.scale;
-        }
-      }
-      __syncthreads();
+      la_exact<DK, 64, 64, TH, true>(a, ss, reinterpret_cast<float*>(tc_smem + T::kK0), row, dir,
+                                     len, lead, h, v0, vcols, decay,
+                                     [&](int i) { return mask[i >> 5] >> (i & 31) & 1; });
       each_state([&](float& held, int r, int col) { held = ss[r * 64 + col]; });
       continue;
     }
