@@ -89,6 +89,10 @@ __device__ __forceinline__ float rsqrt_f(float x) {
   return fmaf(r * 0.5f, fmaf(-x * r, r, 1.f), r);
 }
 
+// Rounding may take a sum of squares below zero; NaN stays (fmaxf would drop
+// it, and with it an infinity among the values).
+__device__ __forceinline__ float at_least_zero(float x) { return x < 0.f ? 0.f : x; }
+
 template <int ACT>
 __device__ __forceinline__ float act_fwd(float z) {
   if (ACT == TTRL_ACT_RELU) return z > 0.f ? z : 0.f;
@@ -598,7 +602,7 @@ __device__ __forceinline__ void block_group_sums(const GnArgs& a, const float* v
 // 1 / count.
 __device__ __forceinline__ float2 mean_rstd(double s1, double s2, double inv, float eps) {
   const double m = s1 * inv;
-  const float var = fmaxf(static_cast<float>(fma(s2, inv, -m * m)), 0.f);
+  const float var = at_least_zero(static_cast<float>(fma(s2, inv, -m * m)));
   return make_float2(static_cast<float>(m), rsqrt_f(var + eps));
 }
 
@@ -686,7 +690,7 @@ __global__ void __launch_bounds__(512) gn_block_kernel(const __grid_constant__ G
           }
           const float d = s * inv;
           mt = x0 + d;
-          q = fmaxf(fmaf(-s, d, q), 0.f);
+          q = at_least_zero(fmaf(-s, d, q));
         }
         if (tid < threads) {
           cols[first + e] = mt;
@@ -942,7 +946,7 @@ __global__ void __launch_bounds__(512, 2) gn_cluster_kernel(const __grid_constan
           const float m = s1[e] * inv;
           const float d = x0[e] + m - mt[e];
           mt[e] = fmaf(d, share, mt[e]);
-          q[e] += fmaxf(fmaf(-s1[e], m, s2[e]), 0.f) + d * d * (cnt * share);
+          q[e] += at_least_zero(fmaf(-s1[e], m, s2[e])) + d * d * (cnt * share);
         }
         cnt = all;
       }
