@@ -39,3 +39,40 @@ def test_a_bad_value_in_any_row_makes_its_group_nan(n, s, c, g, bad):
     wide = hurt[:, None, :, None].expand(n, s, g, c // g).reshape(n * s, c)
     assert bool(torch.isnan(y[wide]).all())
     assert torch.equal(y[~wide], clean[~wide])
+
+
+@gpu
+@pytest.mark.parametrize("n,s,c,g,off", [
+    (9, 16, 32, 4, 0), (9, 80, 32, 4, 0), (9, 80, 32, 4, 1), (160, 400, 90, 6, 0),
+    (3, 5879, 64, 2, 0),
+    (300, 441, 128, 8, 0),  # forward by clusters, backward over global memory
+    (300, 441, 128, 8, 1),  # and by single floats
+])
+def test_a_relu_gate_is_the_forwards(n, s, c, g, off):
+    """Where z is the rounding of a product, the backward opens the gates that
+    the forward opened: dbias counts them (dy is one), and dx is the formula's
+    for them."""
+    gen = torch.Generator("cuda").manual_seed(2)
+    image = torch.randint(-3, 4, (s, c), device="cuda", generator=gen) * 0.37 + 0.11
+    x = image.repeat(n, 1)
+    w = 1.0 + 0.3 * torch.randn(c, device="cuda", generator=gen)
+    y, stats = torch.empty_like(x), torch.empty(n, g, 2, device="cuda")
+    shape = dict(groups=g, spatial=s)
+    _context().group_norm_fwd(x, w, None, y, stats, act="none", **shape)
+    mean, rstd = (stats[0, :, i].repeat_interleave(c // g) for i in (0, 1))
+    hat = (image - mean) * rstd
+    b = -(hat * w)[0]  # z of a seventh of the elements is a rounding
+    _context().group_norm_fwd(x, w, b, y, stats, act="relu", **shape)
+    gate = y > 0
+    near = (image == image[0]).repeat(n, 1)
+    assert 0 < int(gate[near].sum()) < int(near.sum())
+    dy = torch.ones(n * s * c + off, device="cuda")[off:].reshape(n * s, c)
+    dx, dw, db = torch.empty_like(x), torch.empty_like(w), torch.empty_like(b)
+    _context().group_norm_bwd(dy, x, w, b, stats, dx, dw, db, act="relu", **shape)
+    assert torch.equal(db, gate.sum(0).float())
+    d = (gate * w).double().reshape(n, s, g, c // g)
+    hat = hat.double().reshape(1, s, g, c // g)
+    r = rstd.double().reshape(1, 1, g, c // g)
+    want = r * (d - d.mean((1, 3), keepdim=True) - hat * (d * hat).mean((1, 3), keepdim=True))
+    # A wrong gate is off by rstd * w, some 1; roundings by some 2^-20 of it.
+    assert float((dx.double() - want.reshape(n * s, c)).abs().max()) < 1e-4

@@ -111,6 +111,10 @@ __device__ __forceinline__ float act_bwd(float dy, float z) {
   return dy;
 }
 
+// z, by the same roundings in every kernel: a ReLU's gate in the backward is the
+// forward's, whichever of them ran it.
+__device__ __forceinline__ float norm_z(float hat, float w, float b) { return fmaf(hat, w, b); }
+
 // Sum over the `lanes` (a power of two) consecutive lanes a lane belongs to.
 __device__ __forceinline__ float seg_sum(float v, int lanes) {
   for (int o = lanes >> 1; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -287,7 +291,7 @@ __global__ void __launch_bounds__(kGnWarps * 32) gn_warp_kernel(const __grid_con
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           if (EL && e > 0) rstd = g2[group(r, e)];
-          x[r].v[e] = act_fwd<ACT>(fmaf(x[r].v[e] * rstd, w.v[e], b.v[e]));
+          x[r].v[e] = act_fwd<ACT>(norm_z(x[r].v[e] * rstd, w.v[e], b.v[e]));
         }
         x[r].store(a.y + base + j * W);
       }
@@ -319,7 +323,7 @@ __global__ void __launch_bounds__(kGnWarps * 32) gn_warp_kernel(const __grid_con
               rs[r][EL ? e : 0] = g2[group(r, e)];
             }
             const float hat = (x[r].v[e] - m) * rs[r][EL ? e : 0];
-            const float dz = act_bwd<ACT>(dy[BWD ? r : 0].v[e], fmaf(hat, w.v[e], b.v[e]));
+            const float dz = act_bwd<ACT>(dy[BWD ? r : 0].v[e], norm_z(hat, w.v[e], b.v[e]));
             acc_w[BWD ? r : 0][e] = fmaf(dz, hat, acc_w[BWD ? r : 0][e]);
             acc_b[BWD ? r : 0][e] += dz;
             x[r].v[e] = hat;
@@ -485,7 +489,7 @@ __global__ void __launch_bounds__(kGnWarps * 32, R <= 4 ? (BWD ? 2 : 3) : 1)
         if (a.b != nullptr) b.load(a.b + j * 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          x[r].v[e] = act_fwd<ACT>(fmaf(x[r].v[e] * rstd, w.v[e], b.v[e]));
+          x[r].v[e] = act_fwd<ACT>(norm_z(x[r].v[e] * rstd, w.v[e], b.v[e]));
         x[r].store(a.y + base + j * 4);
       }
     } else {
@@ -505,7 +509,7 @@ __global__ void __launch_bounds__(kGnWarps * 32, R <= 4 ? (BWD ? 2 : 3) : 1)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float hat = (x[r].v[e] - mr.x) * mr.y;
-          const float dz = act_bwd<ACT>(dy[BWD ? r : 0].v[e], fmaf(hat, w.v[e], b.v[e]));
+          const float dz = act_bwd<ACT>(dy[BWD ? r : 0].v[e], norm_z(hat, w.v[e], b.v[e]));
           acc_w[BWD ? r : 0][e] = fmaf(dz, hat, acc_w[BWD ? r : 0][e]);
           acc_b[BWD ? r : 0][e] += dz;
           const float d = dz * w.v[e];
@@ -717,7 +721,7 @@ __global__ void __launch_bounds__(512) gn_block_kernel(const __grid_constant__ G
         if (r >= k) continue;
 #pragma unroll
         for (int e = 0; e < W; ++e)
-          x[r].v[e] = act_fwd<ACT>(fmaf((x[r].v[e] - m[e]) * rs[e], w[e], b[e]));
+          x[r].v[e] = act_fwd<ACT>(norm_z((x[r].v[e] - m[e]) * rs[e], w[e], b[e]));
         x[r].store(a.y + base + r * step);
       }
     } else {
@@ -735,7 +739,7 @@ __global__ void __launch_bounds__(512) gn_block_kernel(const __grid_constant__ G
 #pragma unroll
         for (int e = 0; e < W; ++e) {
           const float hat = (x[r].v[e] - m[e]) * rs[e];
-          const float dz = act_bwd<ACT>(dy[BWD ? r : 0].v[e], fmaf(hat, w[e], b[e]));
+          const float dz = act_bwd<ACT>(dy[BWD ? r : 0].v[e], norm_z(hat, w[e], b[e]));
           t1[e] += dz;
           t2[e] = fmaf(dz, hat, t2[e]);
           x[r].v[e] = hat;
@@ -959,12 +963,12 @@ __global__ void __launch_bounds__(512, 2) gn_cluster_kernel(const __grid_constan
       __syncthreads();
       block_group_sums<W, true>(a, cols, cols2, sums, threads, slots, rest);
     } else {
-      float m[W], rs[W], rw[W], b[W], t1[W], t2[W];
+      float m[W], rs[W], w[W], b[W], t1[W], t2[W];
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         m[e] = st[gid(e) * 2];
         rs[e] = st[gid(e) * 2 + 1];
-        rw[e] = a.w != nullptr ? rs[e] * a.w[col(e)] : rs[e];
+        w[e] = a.w != nullptr ? a.w[col(e)] : 1.f;
         b[e] = a.b != nullptr ? a.b[col(e)] : 0.f;
         t1[e] = t2[e] = 0.f;
       }
@@ -981,19 +985,17 @@ __global__ void __launch_bounds__(512, 2) gn_cluster_kernel(const __grid_constan
           if (live(u))
 #pragma unroll
             for (int e = 0; e < W; ++e) {
-              const float d = x[u].v[e] - m[e];
-              const float dz = act_bwd<ACT>(dy[u].v[e], fmaf(d, rw[e], b[e]));
+              const float hat = (x[u].v[e] - m[e]) * rs[e];
+              const float dz = act_bwd<ACT>(dy[u].v[e], norm_z(hat, w[e], b[e]));
               t1[e] += dz;
-              t2[e] = fmaf(dz, d, t2[e]);
+              t2[e] = fmaf(dz, hat, t2[e]);
             }
       });
       if (mine)
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          t2[e] *= rs[e];
-          const float w = a.w != nullptr ? a.w[col(e)] : 1.f;
-          cols[first + e] = t1[e] * w;
-          cols2[first + e] = t2[e] * w;
+          cols[first + e] = t1[e] * w[e];
+          cols2[first + e] = t2[e] * w[e];
           acc[first + e] += t2[e];
           acc[step + first + e] += t1[e];
         }
@@ -1029,12 +1031,13 @@ __global__ void __launch_bounds__(512, 2) gn_cluster_kernel(const __grid_constan
     }
     __syncthreads();
     if (!BWD) {
-      float m[W], rw[W], b[W];
+      float m[W], rs[W], w[W], b[W];
 #pragma unroll
       for (int e = 0; e < W; ++e) {
         const float2 t = merged[gid(e)];
         m[e] = t.x;
-        rw[e] = a.w != nullptr ? t.y * a.w[col(e)] : t.y;
+        rs[e] = t.y;
+        w[e] = a.w != nullptr ? a.w[col(e)] : 1.f;
         b[e] = a.b != nullptr ? a.b[col(e)] : 0.f;
       }
       walk(first, len, [&](auto live, int i) {
@@ -1047,21 +1050,20 @@ __global__ void __launch_bounds__(512, 2) gn_cluster_kernel(const __grid_constan
           if (live(u)) {
 #pragma unroll
             for (int e = 0; e < W; ++e)
-              x[u].v[e] = act_fwd<ACT>(fmaf(x[u].v[e] - m[e], rw[e], b[e]));
+              x[u].v[e] = act_fwd<ACT>(norm_z((x[u].v[e] - m[e]) * rs[e], w[e], b[e]));
             x[u].store_last(ys + i + u * step);
           }
       });
     } else {
-      // dx = dz * (rstd w) - (rstd mean(d)) - (x - mean) * (rstd^2 mean(d hat))
-      float m[W], rw[W], b[W], c1[W], c2[W];
+      float m[W], rs[W], w[W], b[W], m1[W], m2[W];
 #pragma unroll
       for (int e = 0; e < W; ++e) {
-        const float rs = st[gid(e) * 2 + 1];
         m[e] = st[gid(e) * 2];
-        rw[e] = a.w != nullptr ? rs * a.w[col(e)] : rs;
+        rs[e] = st[gid(e) * 2 + 1];
+        w[e] = a.w != nullptr ? a.w[col(e)] : 1.f;
         b[e] = a.b != nullptr ? a.b[col(e)] : 0.f;
-        c1[e] = rs * merged[gid(e)].x;
-        c2[e] = rs * (rs * merged[gid(e)].y);
+        m1[e] = merged[gid(e)].x;
+        m2[e] = merged[gid(e)].y;
       }
       walk(first, len, [&](auto live, int i) {
         Vec<W> x[U], dy[U];
@@ -1076,9 +1078,9 @@ __global__ void __launch_bounds__(512, 2) gn_cluster_kernel(const __grid_constan
           if (live(u)) {
 #pragma unroll
             for (int e = 0; e < W; ++e) {
-              const float d = x[u].v[e] - m[e];
-              const float dz = act_bwd<ACT>(dy[u].v[e], fmaf(d, rw[e], b[e]));
-              x[u].v[e] = fmaf(dz, rw[e], -fmaf(d, c2[e], c1[e]));
+              const float hat = (x[u].v[e] - m[e]) * rs[e];
+              const float dz = act_bwd<ACT>(dy[u].v[e], norm_z(hat, w[e], b[e]));
+              x[u].v[e] = rs[e] * fmaf(-hat, m2[e], fmaf(dz, w[e], -m1[e]));
             }
             x[u].store_last(ys + i + u * step);
           }
@@ -1190,7 +1192,7 @@ __global__ void __launch_bounds__(kGnWideThreads)
 #pragma unroll
           for (int e = 0; e < W; ++e) {
             const float hat = (x[i].v[e] - m[e]) * rs[e];
-            const float dz = act_bwd<ACT>(dy[i].v[e], fmaf(hat, w[e], b[e]));
+            const float dz = act_bwd<ACT>(dy[i].v[e], norm_z(hat, w[e], b[e]));
             s1[e] += dz;
             s2[e] = fmaf(dz, hat, s2[e]);
           }
@@ -1315,16 +1317,16 @@ __global__ void __launch_bounds__(kGnWideThreads)
   const int n = blockIdx.x / p.splits;
   const int r0 = split * p.rows;
   const int r1 = min(a.spatial, r0 + p.rows);
-  float m[W], rw[W], b[W], c1[W], c2[W];
+  float m[W], rs[W], w[W], b[W], m1[W], m2[W];
 #pragma unroll
   for (int e = 0; e < W; ++e) {
     const long long id = static_cast<long long>(n) * a.groups + fdiv(a.f_cg, c + e);
-    const float rs = a.stats[id * 2 + 1];
     m[e] = a.stats[id * 2];
-    rw[e] = a.w != nullptr ? rs * a.w[c + e] : rs;
+    rs[e] = a.stats[id * 2 + 1];
+    w[e] = a.w != nullptr ? a.w[c + e] : 1.f;
     b[e] = a.b != nullptr ? a.b[c + e] : 0.f;
-    c1[e] = BWD ? rs * p.group[id * 2] : 0.f;
-    c2[e] = BWD ? rs * (rs * p.group[id * 2 + 1]) : 0.f;
+    m1[e] = BWD ? p.group[id * 2] : 0.f;
+    m2[e] = BWD ? p.group[id * 2 + 1] : 0.f;
   }
   const long long base = static_cast<long long>(n) * a.spatial * a.channels + c;
   constexpr int U = 4;
@@ -1342,9 +1344,9 @@ __global__ void __launch_bounds__(kGnWideThreads)
       if (r + i * p.down < r1) {
 #pragma unroll
         for (int e = 0; e < W; ++e) {
-          const float d = x[i].v[e] - m[e], z = fmaf(d, rw[e], b[e]);
+          const float hat = (x[i].v[e] - m[e]) * rs[e], z = norm_z(hat, w[e], b[e]);
           if (BWD)
-            x[i].v[e] = fmaf(act_bwd<ACT>(dy[i].v[e], z), rw[e], -fmaf(d, c2[e], c1[e]));
+            x[i].v[e] = rs[e] * fmaf(-hat, m2[e], fmaf(act_bwd<ACT>(dy[i].v[e], z), w[e], -m1[e]));
           else
             x[i].v[e] = act_fwd<ACT>(z);
         }
