@@ -1,6 +1,9 @@
 """Group norm where its plans (a warp, a block, a cluster an image, passes over
 global memory) have to agree."""
 
+import subprocess
+import sys
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -76,3 +79,37 @@ def test_a_relu_gate_is_the_forwards(n, s, c, g, off):
     want = r * (d - d.mean((1, 3), keepdim=True) - hat * (d * hat).mean((1, 3), keepdim=True))
     # A wrong gate is off by rstd * w, some 1; roundings by some 2^-20 of it.
     assert float((dx.double() - want.reshape(n * s, c)).abs().max()) < 1e-4
+
+
+_PROBE = """
+import hashlib, sys
+sys.path.insert(0, "tt-rl_b200")
+import torch
+from ttrl_b200.device import context
+ctx = context("cuda:0")
+
+def backward(n, s, c, g):
+    gen = torch.Generator("cuda").manual_seed(3)
+    x, dy = (torch.randn(n * s, c, device="cuda", generator=gen) for _ in range(2))
+    y, stats = torch.empty_like(x), torch.empty(n, g, 2, device="cuda")
+    ctx.group_norm_fwd(x, None, None, y, stats, groups=g, spatial=s)
+    dw, db = torch.empty(c, device="cuda"), torch.empty(c, device="cuda")
+    ctx.group_norm_bwd(dy, x, None, None, stats, y, dw, db, groups=g, spatial=s)
+    return hashlib.sha1(b"".join(t.cpu().numpy().tobytes() for t in (y, dw, db))).hexdigest()
+
+shapes = {"narrow": (1200, 441, 96, 3), "wide": (800, 32, 2048, 8)}
+print({name: backward(*shapes[name]) for name in sys.argv[1:]}["narrow"])
+"""
+
+
+@gpu
+def test_results_do_not_depend_on_the_shapes_before():
+    """Clusters of 256 and of 512 threads: how many are resident, and so which
+    images a column's sums are added up by, is each kind's own."""
+    def first(*names):
+        run = subprocess.run([sys.executable, "-c", _PROBE, *names], capture_output=True,
+                             text=True, timeout=300)
+        assert run.returncode == 0, run.stderr
+        return run.stdout.strip().splitlines()[-1]
+
+    assert first("narrow") == first("wide", "narrow")

@@ -1618,15 +1618,16 @@ static cudaError_t launch_cluster(const GnPlan& p, const GnArgs& a, int* partial
                                   cudaStream_t st) {
   // Clusters that are resident at once: fewer than the SM count says where
   // they do not pack into the GPCs. Asked once per device for each cluster
-  // size and number of CTAs an SM.
+  // size, and number of CTAs an SM by their shared memory and threads: how an
+  // image falls to a cluster depends on the call's shape only.
   static std::mutex lock;
   static bool ready[64] = {};
-  static int known[64][kGnMaxCluster + 1][2] = {};
+  static int known[64][kGnMaxCluster + 1][2][2] = {};
   const auto kernel = gn_cluster_kernel<W, ACT, BWD, STAGED>;
-  const bool wide = p.smem > 56 * 1024;
+  const bool wide = p.smem > 56 * 1024, many = p.threads > 256;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(p.ctas);
-  cfg.blockDim = dim3(p.threads > 256 ? 512 : 256);
+  cfg.blockDim = dim3(many ? 512 : 256);
   cfg.dynamicSmemBytes = wide ? kGnSmemMax : 56 * 1024;
   cfg.stream = st;
   cudaLaunchAttribute attr[2];
@@ -1650,12 +1651,12 @@ static cudaError_t launch_cluster(const GnPlan& p, const GnArgs& a, int* partial
       if (e != cudaSuccess) return e;
       ready[dev] = true;
     }
-    most = known[dev][p.ctas][wide];
+    most = known[dev][p.ctas][wide][many];
     if (most == 0) {
       e = cudaOccupancyMaxActiveClusters(&most, kernel, &cfg);
       if (e != cudaSuccess) return e;
       if (most < 1) most = 1;
-      known[dev][p.ctas][wide] = most;
+      known[dev][p.ctas][wide][many] = most;
     }
   }
   // As many images for each cluster: one more round for a few of them would
