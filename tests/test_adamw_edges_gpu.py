@@ -1,0 +1,34 @@
+"""AdamW at the edges: 8-bit codes of blocks whose scale is near either end of
+float's range, rates that float cannot hold, parameters changed in place, and
+clipping over more tensors than one launch of the norm takes."""
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+from tests.test_adamw_gpu import HYPER, leaves, pack_plain  # noqa: E402
+
+gpu = pytest.mark.gpu
+
+
+@gpu
+@pytest.mark.parametrize("scale", [3e38, 1e38, 2.0 ** 126, 2.0 ** 125, 1e-30, 1e-38, 1e-40, 3e-45])
+def test_codes_of_very_large_and_small_blocks(scale):
+    """Bit for bit those of IEEE arithmetic: 1 / scale runs out of float's range
+    at both ends."""
+    from ttrl_b200.engine.optim import AdamW
+    ps = leaves([1024], 5)
+    opt = AdamW(ps, state_bits=8, min_8bit_size=1, **HYPER)
+    rng = np.random.default_rng(6)
+    share = rng.uniform(-1, 1, 1024).astype(np.float32)
+    share[::256] = 1.0
+    m = (share * np.float32(scale)).astype(np.float32)
+    v = np.abs(m)
+    assert np.isfinite(m).all()
+    opt.load_moments([torch.from_numpy(m).cuda()], [torch.from_numpy(v).cuda()], t=1)
+    for codes, scales, x, signed in ((opt._m8, opt._m_scale, m, True),
+                                     (opt._v8, opt._v_scale, v, False)):
+        want, size = pack_plain(x, signed)
+        assert np.array_equal(codes.cpu().numpy().astype(np.int32)[:1024], want)
+        assert np.array_equal(scales.cpu().numpy(), size)

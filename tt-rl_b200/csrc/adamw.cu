@@ -166,10 +166,11 @@ __device__ __forceinline__ void put4(float* p, long long i, long long end, bool 
 // whole blocks, so a word never leaves them.
 __device__ __forceinline__ void put_codes(uint8_t* m8, uint8_t* v8, const float (&m)[2][4],
                                           const float (&v)[2][4], float mm, float vm) {
-  // A scale too small to invert gives infinities, and those are in doubt.
+  // A scale too small to invert gives infinities, and those are in doubt; one
+  // above 2^126 gives zero, by the fast quotient's definition, and so is that.
   const float minv = mm > 0.f ? __fdividef(1.f, mm) : 0.f;
   const float vinv = vm > 0.f ? __fdividef(1.f, vm) : 0.f;
-  bool doubt = false;
+  bool doubt = fmaxf(mm, vm) > 0x1p126f;
   uint32_t mc[2], vc[2];
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
