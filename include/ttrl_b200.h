@@ -331,7 +331,8 @@ typedef struct {
  *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * The step uses the new moments before they are rounded to codes. steps,
  * ticket, grad_scale and bias_table are ttrl_adam_step's; lr_device (one
- * device double, may be NULL) overrides lr at execution time. A value that is
+ * device double, may be NULL) overrides lr at execution time. eps is at least
+ * 2^-126, as the quotient is a float's. A value that is
  * not finite makes its block's 8-bit moments NaN. No reference counterpart
  * (its Adam adds the decay to the gradient, ttrl/engine/optim/adam.py:110-113). */
 int ttrl_adamw_step(const ttrl_adamw_tensor* tensors, int count, int32_t* steps, int32_t* ticket,

@@ -32,3 +32,23 @@ def test_codes_of_very_large_and_small_blocks(scale):
         want, size = pack_plain(x, signed)
         assert np.array_equal(codes.cpu().numpy().astype(np.int32)[:1024], want)
         assert np.array_equal(scales.cpu().numpy(), size)
+
+
+@gpu
+def test_an_eps_below_floats_range_is_refused():
+    """The kernel divides in float: an eps that is zero there would make NaN of
+    every parameter whose gradients have been zero."""
+    from ttrl_b200.engine.optim import AdamW
+    ps = leaves([300], 7)
+    for eps in (1e-50, 1e-40, 2.0 ** -127):
+        with pytest.raises(ValueError, match="eps"):
+            AdamW(ps, lr=1e-3, eps=eps)
+    opt = AdamW(ps, lr=1e-3, eps=2.0 ** -126, weight_decay=0.0)
+    before = ps[0].data.clone()
+    ps[0].grad = torch.zeros_like(before)
+    opt.step()
+    assert torch.equal(ps[0].data, before)
+    state = opt.state_dict()
+    state["eps"] = 1e-50
+    with pytest.raises(ValueError, match="eps"):
+        opt.load_state_dict(state)

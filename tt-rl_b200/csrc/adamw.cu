@@ -459,7 +459,9 @@ int adamw_step(const ttrl_adamw_tensor* tensors, int count, int32_t* steps, int3
     return set_error(TTRL_EINVAL, "adamw: null tensor list, step counter or ticket");
   if (!(b1 >= 0.0 && b1 < 1.0 && b2 >= 0.0 && b2 < 1.0))
     return set_error(TTRL_EINVAL, "adamw: betas have to be in [0, 1)");
-  if (!(eps > 0.0)) return set_error(TTRL_EINVAL, "adamw: eps has to be positive");
+  // The step divides by sqrt(v) + eps in float, of which 1 / eps has to be one.
+  if (!(eps >= 0x1p-126))
+    return set_error(TTRL_EINVAL, "adamw: eps has to be at least 2^-126, got %g", eps);
   if (!(wd >= 0.0)) return set_error(TTRL_EINVAL, "adamw: weight decay has to be >= 0");
   for (int i = 0; i < count; ++i) {
     const ttrl_adamw_tensor& t = tensors[i];

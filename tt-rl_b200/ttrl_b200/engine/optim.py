@@ -42,6 +42,9 @@ def adam_fused_scalars(lr: float, b1: float, b2: float, eps: float, t: int) -> t
 #: back to the kernel's own pow().
 BIAS_TABLE_MAX_STEPS = 1 << 20
 
+#: AdamW's smallest eps: the smallest normal float32.
+EPS_MIN = 2.0 ** -126
+
 _BIAS_TABLES: dict = {}
 
 
@@ -381,8 +384,9 @@ class AdamW(Optimizer):
         b1, b2 = betas
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
             raise ValueError(f"AdamW: betas must be in [0, 1), got {betas}")
-        if not eps > 0:
-            raise ValueError(f"AdamW: eps must be > 0, got {eps}")
+        if not eps >= EPS_MIN:
+            raise ValueError(f"AdamW: eps must be at least 2^-126 (the step divides in float32), "
+                             f"got {eps}")
         if not weight_decay >= 0:
             raise ValueError(f"AdamW: weight_decay must be >= 0, got {weight_decay}")
         if state_bits not in (8, 32):
@@ -647,7 +651,7 @@ class AdamW(Optimizer):
                              f"expected {count}.")
         if t < 0 or any(s < 0 for s in steps):
             raise ValueError(f"AdamW.load_state_dict: step counts must be >= 0, got t={t}.")
-        if not (lr > 0 and eps > 0 and weight_decay >= 0 and 0.0 <= b1 < 1.0
+        if not (lr > 0 and eps >= EPS_MIN and weight_decay >= 0 and 0.0 <= b1 < 1.0
                 and 0.0 <= b2 < 1.0):
             raise ValueError(f"AdamW.load_state_dict: lr={lr}, betas={(b1, b2)}, eps={eps} or "
                              f"weight_decay={weight_decay} is out of range.")
