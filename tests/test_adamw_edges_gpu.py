@@ -52,3 +52,25 @@ def test_an_eps_below_floats_range_is_refused():
     state["eps"] = 1e-50
     with pytest.raises(ValueError, match="eps"):
         opt.load_state_dict(state)
+
+
+@gpu
+@pytest.mark.parametrize("change", ["transposed", "moved over another", "dtype"])
+def test_a_parameter_changed_in_place_is_refused(change):
+    """The same tensor object, with other strides, memory or type: refused
+    before anything is written."""
+    from ttrl_b200.engine.optim import AdamW
+    ps = leaves([(64, 64), (64, 64), 100], 8)
+    opt = AdamW(ps, **HYPER)
+    opt.step()
+    if change == "transposed":
+        ps[0].data.t_()
+    elif change == "moved over another":
+        ps[0].data.set_(ps[1].data)
+    else:
+        ps[0].data.data = torch.zeros(64, 64, device="cuda", dtype=torch.int32)
+    before = [p.data.clone() for p in ps]
+    with pytest.raises(ValueError, match="AdamW"):
+        opt.step()
+    assert all(torch.equal(p.data, b) for p, b in zip(ps, before))
+    assert opt.steps == [1, 1, 1]

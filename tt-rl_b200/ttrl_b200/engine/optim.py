@@ -454,6 +454,7 @@ class AdamW(Optimizer):
         self.grad_scale = None
         self.captured_indices: list[int] | None = None
         self._seen: list = []
+        self._seen_at = np.zeros(0, np.uint64)
         self._all = list(range(len(self.params)))
         self._any_empty = not all(self._numels)
         self._bias = adam_bias_table(self.b1, self.b2, dev)
@@ -490,21 +491,24 @@ class AdamW(Optimizer):
         if not all(map(torch.Tensor.is_contiguous, grads)):
             grads = [g.contiguous() for g in grads]  # held until the launch is issued
         self._look_over("gradient", grads, numels, stepped)
-        # The parameters are looked over again when one has been rebound or resized.
+        at = np.frombuffer(array("Q", map(torch.Tensor.data_ptr, chain(datas, grads))),
+                           np.uint64)
+        where = at[:len(datas)]
+        # The parameters are looked over again when one has been rebound, moved
+        # or resized.
         if (len(datas) != len(self._seen) or not all(map(operator.is_, datas, self._seen))
+                or not np.array_equal(where, self._seen_at)
                 or list(map(torch.Tensor.numel, datas)) != numels):
             self._look_over("data", datas, numels, stepped)
-            if not all(map(torch.Tensor.is_contiguous, datas)):
-                raise ValueError("AdamW: a parameter was rebound to a strided view")
             self._keep_apart(datas)
-            self._seen = datas
+            self._seen, self._seen_at = datas, where
+        if not all(map(torch.Tensor.is_contiguous, datas)):
+            raise ValueError("AdamW: a parameter has become a strided view")
         if stepped:
             table = self._table
             if len(stepped) < len(table):
                 table = table[stepped]
-            at = np.frombuffer(array("Q", map(torch.Tensor.data_ptr, chain(datas, grads))),
-                               np.uint64)
-            table["param"], table["grad"] = at[:len(datas)], at[len(datas):]
+            table["param"], table["grad"] = where, at[len(datas):]
             context(self._device).adamw_step(
                 table, self._dev_steps, self._ticket, self.grad_scale, self._lr, self.b1,
                 self.b2, self.eps, self.weight_decay, lr_device=self._lr_dev, bias=self._bias)
