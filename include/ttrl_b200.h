@@ -359,7 +359,8 @@ int ttrl_adamw_state_convert(const ttrl_adamw_state* tensors, int count, int pac
  * grad_sq_device at :46-61). When max_norm > 0 also writes
  * out[1] = max_norm/(norm+1e-6) if norm > max_norm else 1, the clip factor
  * of clip_grad_norm (ttrl/algos/grads.py:29-43). `grads`/`numels` are host
- * arrays of device pointers and counts; `out` is a device float[2];
+ * arrays of device pointers and counts, of any length (a launch for every
+ * TTRL_ADAM_MAX_TENSORS); `out` is a device float[2];
  * `workspace` needs ttrl_grad_sqnorm_workspace_bytes and must start zeroed
  * (the kernel leaves its ticket zero). */
 int ttrl_grad_sqnorm(const float* const* grads, const int64_t* numels, int count, float* out,

@@ -74,3 +74,45 @@ def test_a_parameter_changed_in_place_is_refused(change):
         opt.step()
     assert all(torch.equal(p.data, b) for p, b in zip(ps, before))
     assert opt.steps == [1, 1, 1]
+
+
+@gpu
+@pytest.mark.parametrize("count", [64, 65, 130, 400])
+def test_clipping_over_many_tensors(count):
+    """The norm of any number of gradients, and a clipped step of AdamW. The sum
+    of squares is in 64 bits; the factor and out[0] are rounded to float once
+    (2^-24), as is each scaled gradient."""
+    from ttrl_b200.algos.grads import clip_grad_norm_device, grad_sq_device
+    from ttrl_b200.engine.optim import AdamW
+    sizes = [1 + 37 * (i % 91) for i in range(count)]
+    sizes[-1] = 100_003
+    ps, twins = leaves(sizes, 9), leaves(sizes, 9)
+    exact = sum(float((p.grad.double() ** 2).sum()) for p in ps)
+    assert abs(float(grad_sq_device(ps)) / exact - 1) <= 2.0 ** -23
+    opt, ref = AdamW(ps, **HYPER), AdamW(twins, **HYPER)
+    out = clip_grad_norm_device(ps, 0.5, opt)
+    factor = 0.5 / (exact ** 0.5 + 1e-6)
+    assert abs(float(out[0]) / exact - 1) <= 2.0 ** -23
+    assert abs(float(out[1]) / factor - 1) <= 2.0 ** -23
+    opt.step()
+    for p in twins:
+        p.grad = p.grad * out[1]
+    ref.step()
+    for p, q in zip(ps, twins):
+        assert torch.equal(p.data, q.data)
+    again = clip_grad_norm_device(ps, 0.5)
+    assert torch.equal(out, again)
+
+
+@gpu
+def test_clipping_passes_over_empty_tensors_and_replays():
+    from ttrl_b200.algos.grads import clip_grad_norm_device
+    ps = leaves([5] * 70 + [0], 10)
+    want = clip_grad_norm_device(ps[:-1], 0.1).clone()
+    assert torch.equal(clip_grad_norm_device(ps, 0.1), want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = clip_grad_norm_device(ps, 0.1)
+    ps[3].grad.mul_(1.0)
+    graph.replay()
+    assert torch.equal(got, want)

@@ -289,7 +289,8 @@ struct SqArgs {
   long long chunk_start[TTRL_ADAM_MAX_TENSORS + 1];
   uint64_t vec_mask;
   int count;
-  int pad0;
+  int last;         // the launch that adds up
+  long long first;  // blocks of the launches before
   double* partial;  // one per block
   int32_t* ticket;
   float* out;
@@ -335,8 +336,11 @@ __global__ void __launch_bounds__(kSqThreads) sqnorm_kernel(const __grid_constan
   }
   const double block_total = block_sum_fixed(s, red);
   if (threadIdx.x == 0) {
-    a.partial[blockIdx.x] = block_total;
-    __threadfence();
+    a.partial[a.first + blockIdx.x] = block_total;
+    if (a.last) __threadfence();
+  }
+  if (!a.last) return;
+  if (threadIdx.x == 0) {
     const unsigned int prev = atomicAdd(reinterpret_cast<unsigned int*>(a.ticket), 1u);
     s_last = prev == gridDim.x - 1;
   }
@@ -347,7 +351,8 @@ __global__ void __launch_bounds__(kSqThreads) sqnorm_kernel(const __grid_constan
   // not depend on which block finished last.
   __threadfence();
   double t = 0.0;
-  for (unsigned int b = threadIdx.x; b < gridDim.x; b += kSqThreads) t += __ldcg(a.partial + b);
+  const long long blocks = a.first + gridDim.x;
+  for (long long b = threadIdx.x; b < blocks; b += kSqThreads) t += __ldcg(a.partial + b);
   const double total = block_sum_fixed(t, red);
   if (threadIdx.x == 0) {
     a.out[0] = static_cast<float>(total);
@@ -370,34 +375,42 @@ size_t sqnorm_ws_bytes(const int64_t* numels, int count) {
 int grad_sqnorm(const float* const* grads, const int64_t* numels, int count, float* out,
                 float max_norm, void* ws, size_t wsb, cudaStream_t st) {
   if (count <= 0) return set_error(TTRL_EINVAL, "grad_sqnorm: no tensors");
-  if (count > TTRL_ADAM_MAX_TENSORS)
-    return set_error(TTRL_EINVAL, "grad_sqnorm: %d tensors exceeds the limit %d", count,
-                     TTRL_ADAM_MAX_TENSORS);
+  for (int i = 0; i < count; ++i)
+    if (numels[i] <= 0 || grads[i] == nullptr)
+      return set_error(TTRL_EINVAL, "grad_sqnorm: tensor %d is empty or null", i);
   const size_t need = sqnorm_ws_bytes(numels, count);
   if (ws == nullptr || wsb < need)
     return set_error(TTRL_EWORKSPACE, "grad_sqnorm: needs %zu bytes of workspace, got %zu",
                      need, wsb);
-  SqArgs a;
-  std::memset(&a, 0, sizeof(a));
-  long long chunks = 0;
-  for (int i = 0; i < count; ++i) {
-    if (numels[i] <= 0 || grads[i] == nullptr)
-      return set_error(TTRL_EINVAL, "grad_sqnorm: tensor %d is empty or null", i);
-    a.g[i] = grads[i];
-    if (al16(grads[i])) a.vec_mask |= 1ull << i;
-    a.numel[i] = numels[i];
-    a.chunk_start[i] = chunks;
-    chunks += (numels[i] + kSqChunk - 1) / kSqChunk;
+  // Launches of as many tensors as the parameters hold, in order: each leaves its
+  // blocks' sums behind those before, the last one's last block adds them all up.
+  long long before = 0;
+  for (int at = 0; at < count; at += TTRL_ADAM_MAX_TENSORS) {
+    SqArgs a;
+    std::memset(&a, 0, sizeof(a));
+    a.count = count - at < TTRL_ADAM_MAX_TENSORS ? count - at : TTRL_ADAM_MAX_TENSORS;
+    long long chunks = 0;
+    for (int i = 0; i < a.count; ++i) {
+      a.g[i] = grads[at + i];
+      if (al16(grads[at + i])) a.vec_mask |= 1ull << i;
+      a.numel[i] = numels[at + i];
+      a.chunk_start[i] = chunks;
+      chunks += (numels[at + i] + kSqChunk - 1) / kSqChunk;
+    }
+    a.chunk_start[a.count] = chunks;
+    a.first = before;
+    a.last = at + a.count == count;
+    a.ticket = static_cast<int32_t*>(ws);
+    a.partial = reinterpret_cast<double*>(static_cast<char*>(ws) + 16);
+    a.out = out;
+    a.max_norm = max_norm;
+    const cudaError_t e = launch_pdl(sqnorm_kernel, dim3(static_cast<unsigned>(chunks)),
+                                     dim3(kSqThreads), 0, st, a);
+    note_launch();
+    if (e != cudaSuccess) return set_cuda_error("grad_sqnorm launch", e);
+    before += chunks;
   }
-  a.chunk_start[count] = chunks;
-  a.count = count;
-  a.ticket = static_cast<int32_t*>(ws);
-  a.partial = reinterpret_cast<double*>(static_cast<char*>(ws) + 16);
-  a.out = out;
-  a.max_norm = max_norm;
-  const cudaError_t le_ = launch_pdl(sqnorm_kernel, dim3(static_cast<unsigned>(chunks)), dim3(kSqThreads), 0, st, a);
-  note_launch();
-  cudaError_t e = le_ != cudaSuccess ? le_ : cudaGetLastError();
+  const cudaError_t e = cudaGetLastError();
   return e == cudaSuccess ? TTRL_OK : set_cuda_error("grad_sqnorm launch", e);
 }
 

@@ -22,7 +22,7 @@ _WS: dict = {}
 
 def _grads(params):
     return [p.grad.reshape(-1) if p.grad.is_contiguous() else p.grad.contiguous().reshape(-1)
-            for p in params if p.grad is not None]
+            for p in params if p.grad is not None and p.grad.numel()]
 
 
 def _sqnorm(params, max_norm: float):
@@ -42,10 +42,7 @@ def _sqnorm(params, max_norm: float):
         ws = torch.zeros(need, dtype=torch.uint8, device=dev)
         _WS[key] = ws
     out = torch.empty(2, dtype=torch.float32, device=dev)
-    for start in range(0, len(grads), 64):
-        if start:
-            raise ValueError("grad-norm over more than 64 tensors is not supported")
-        ctx.grad_sqnorm(grads[start:start + 64], out, max_norm, ws)
+    ctx.grad_sqnorm(grads, out, max_norm, ws)
     return out
 
 

@@ -466,8 +466,6 @@ class DeviceContext:
                                                      self.stream), "ttrl_adamw_state_convert")
 
     def grad_sqnorm(self, grads, out, max_norm: float, workspace) -> None:
-        if len(grads) > 64:
-            raise ValueError("grad_sqnorm: more than 64 tensors per call")
         ptrs = (ctypes.c_void_p * len(grads))(*[_ptr(_f32(g, "grad")) for g in grads])
         numels = (ctypes.c_int64 * len(grads))(*[g.numel() for g in grads])
         need = lib().ttrl_grad_sqnorm_workspace_bytes(numels, len(grads))
