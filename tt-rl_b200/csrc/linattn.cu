@@ -1899,7 +1899,9 @@ int linear_attention_step(const float* qkv, const float* s_in, const float* star
     return set_error(TTRL_EINVAL, "linear_attention_step: null pointer");
   const int64_t state = static_cast<int64_t>(batch) * heads * kd * vd;
   const Span in[] = {{"qkv", qkv, static_cast<int64_t>(batch) * heads * (2 * kd + vd)},
-                       {"state", s_out == s_in ? nullptr : s_in, state}};
+                       {"state", s_out == s_in ? nullptr : s_in, state},
+                       {"starts", starts, batch},
+                       {"decay", decay, heads}};
   const Span made[] = {{"out", out, static_cast<int64_t>(batch) * heads * vd},
                          {"new_state", s_out, state}};
   if ((rc = spans_apart("linear_attention_step", in, made))) return rc;
@@ -1940,7 +1942,10 @@ int linear_attention_fwd(const float* qkv, const float* s_in, const float* start
   const int64_t state = static_cast<int64_t>(batch) * heads * kd * vd;
   // Results are written while other blocks, and the scans that follow, still
   // read what came in.
-  const Span in[] = {{"qkv", qkv, rows * heads * (2 * kd + vd)}, {"state", s_in, state}};
+  const Span in[] = {{"qkv", qkv, rows * heads * (2 * kd + vd)},
+                     {"state", s_in, state},
+                     {"starts", starts, rows},
+                     {"decay", decay, heads}};
   const Span made[] = {{"out", out, rows * heads * vd}, {"new_state", s_out, state}};
   char* room = nullptr;
   if ((rc = la_workspace("linear_attention_fwd", steps, batch, heads, kd, vd, ws, ws_bytes, &room)))
@@ -1977,7 +1982,9 @@ int linear_attention_bwd(const float* dout, const float* ds_out, const float* qk
   const Span in[] = {{"qkv", qkv, rows * heads * (2 * kd + vd)},
                        {"state", s_in, state},
                        {"dout", dout, rows * heads * vd},
-                       {"dnew_state", ds_out, state}};
+                       {"dnew_state", ds_out, state},
+                       {"starts", starts, rows},
+                       {"decay", decay, heads}};
   const Span made[] = {{"dqkv", dqkv, rows * heads * (2 * kd + vd)}, {"dstate", ds_in, state}};
   char* room = nullptr;
   if ((rc = la_workspace("linear_attention_bwd", steps, batch, heads, kd, vd, ws, ws_bytes, &room)))
