@@ -1,6 +1,8 @@
 """Linear attention: results over its flags and decays, rows wider than 32-bit
 offsets, and states that stay infinite over long sequences."""
 
+import ctypes
+
 import pytest
 
 torch = pytest.importorskip("torch")
@@ -42,3 +44,23 @@ def test_results_over_flags_and_decays_are_refused(name):
             else:
                 ctx.linear_attention_bwd(dout, None, qkv, state, starts, decay, dqkv, new,
                                          **shape)
+
+
+def test_rows_beyond_32_bit_offsets_are_refused():
+    """Offsets within a row are 32 bits: a row of 2^31 floats or more is refused
+    by its extents alone (no pointer is looked at)."""
+    from ttrl_b200._lib import lib
+    p, null = ctypes.c_void_p(64), None
+    for heads, kd, vd in ((1 << 24, 128, 1), (1 << 23, 64, 128), (1 << 24, 1, 126)):
+        assert heads * (2 * kd + vd) >= 1 << 31
+        assert lib().ttrl_linear_attention_workspace_bytes(2, 1, heads, kd, vd) == 0
+        calls = (
+            lambda: lib().ttrl_linear_attention_fwd(p, null, null, p, p, null, 2, 1, heads, kd,
+                                                    vd, 1.0, null, 0, null),
+            lambda: lib().ttrl_linear_attention_bwd(p, null, p, null, null, p, p, null, 2, 1,
+                                                    heads, kd, vd, 1.0, null, 0, null),
+            lambda: lib().ttrl_linear_attention_step(p, p, null, p, p, p, 1, heads, kd, vd, 1.0,
+                                                     null))
+        for call in calls:
+            assert call() != 0
+            assert b"row" in lib().ttrl_last_error()

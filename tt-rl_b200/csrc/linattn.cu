@@ -1835,6 +1835,9 @@ static int la_check(const char* what, int steps, int batch, int heads, int kd, i
   if (static_cast<long long>(batch) * heads * kd * vd >= (1ll << 39) ||
       static_cast<long long>(batch) * heads >= (1ll << 31))
     return set_error(TTRL_EUNSUPPORTED, "%s: too many lanes and heads", what);
+  // A head's place in its row is a 32-bit number.
+  if (static_cast<long long>(heads) * (2 * kd + vd) >= (1ll << 31))
+    return set_error(TTRL_EUNSUPPORTED, "%s: a row of 2^31 values or more", what);
   return TTRL_OK;
 }
 
