@@ -64,3 +64,33 @@ def test_rows_beyond_32_bit_offsets_are_refused():
         for call in calls:
             assert call() != 0
             assert b"row" in lib().ttrl_last_error()
+
+
+@gpu
+@pytest.mark.parametrize("decay", [0.9, 0.5, 0.0])
+@pytest.mark.parametrize("t", [700, 9000])
+def test_an_infinite_state_stays_infinite(t, decay):
+    """decay * inf is inf for every decay but zero, however long the sequence
+    (its power over a part of it may be zero in float)."""
+    from ttrl_b200.device import context
+    ctx = context("cuda:0")
+    kd = vd = 64
+    g = torch.Generator("cuda").manual_seed(4)
+    qkv = torch.randn(t, 1, 2 * kd + vd, device="cuda", generator=g)
+    state = torch.randn(1, 1, kd, vd, device="cuda", generator=g)
+    state[0, 0, 3, 5], state[0, 0, 7, 9] = float("inf"), float("-inf")
+    d = torch.tensor([decay], device="cuda")
+    out, new = torch.empty(t, 1, vd, device="cuda"), torch.empty_like(state)
+    shape = dict(heads=1, key_dim=kd, value_dim=vd, scale=0.1)
+    ctx.linear_attention_fwd(qkv, state, None, d, out, new, **shape)
+    want = torch.zeros_like(state)
+    want[0, 0, 3, 5], want[0, 0, 7, 9] = (float("inf") * decay, float("-inf") * decay)
+    bad = ~torch.isfinite(want)
+    assert torch.equal(torch.isfinite(new), ~bad)
+    torch.testing.assert_close(new[bad], want[bad], rtol=0, atol=0, equal_nan=True)
+    columns = torch.ones(vd, dtype=torch.bool, device="cuda")
+    columns[[5, 9]] = False
+    assert torch.isfinite(out[:, 0, columns]).all()
+    q = qkv[:, 0, [3, 7]]
+    first = torch.stack([q[:, 0] * want[0, 0, 3, 5], q[:, 1] * want[0, 0, 7, 9]], 1)
+    torch.testing.assert_close(out[:, 0, [5, 9]], first, rtol=0, atol=0, equal_nan=True)

@@ -1553,6 +1553,8 @@ __global__ void __launch_bounds__(128) la_join_kernel(const __grid_constant__ La
       const int len = min(a.sum_len, a.steps - q * a.sum_len);
       if (q == 0 && a.reverse) f = decay_pow(lg, len - 1);
       else if (len < a.sum_len) f = decay_pow(lg, len);
+      // A power that float cannot hold is no zero to an infinite state.
+      if (f == 0.f && a.decay[h] > 0.f && isinf(s)) f = 1.f;
       s = cut[u] ? own[u] : fmaf(f, s, own[u]);
       if ((q + 1) % sub == 0) a.seg[q * all + i] = s;
     }
