@@ -162,3 +162,22 @@ def test_ordinary_sequences_beside_uneven_ones():
     for lane in (0, 2):
         assert torch.equal(alone[0][:, lane], beside[0][:, lane])
         assert torch.equal(alone[1][lane], beside[1][lane])
+
+
+@gpu
+@pytest.mark.parametrize("sizes", [dict(dout=1e-20, dstate=1e-20), dict(k=1e-24), dict(v=1e-30),
+                                   dict(k=1e-17, v=1e-17), dict(q=1e-15, k=1e-17)])
+@pytest.mark.parametrize("t,b,h,kd,vd", SHAPES)
+def test_tiny_operands_keep_their_bits(t, b, h, kd, vd, sizes):
+    """Whole operands, down to what fp32 itself holds (a state of 1e-34)."""
+    d = draw(t, b, h, kd, vd)
+    d["state"] *= 0
+    d["dstate"] *= 0 if "dout" not in sizes else 1
+    for name, size in sizes.items():
+        d[name] *= size
+    pairs = run(d)
+    near(pairs["out"], -1)
+    near(pairs["new"], (-1, -2))
+    near(pairs["first"], (-1, -2))
+    for name in ("dq", "dk", "dv"):
+        near(pairs[name], -1)

@@ -31,7 +31,8 @@
 // token's error goes by what its own result is made of, not by a larger token in
 // the same tile, in an episode that a start has dropped or later in time. (One
 // power a tile took 13% less time, and lost all bits of a token beside one 10^12
-// times its size; done in fp32, a chunk takes ten times as long.) A product is
+// times its size; done in fp32, a chunk takes ten times as long. Tokens of e^N(0, 1)
+// times a size each: 638 us instead of 637 backward; of e^3N(0, 1), 728.) A product is
 // hi hi + hi lo + lo hi, three mma.sync of 16-bit operands at twice the rate
 // that two-part tf32 has. k, v and the state are split once, as they are
 // stored in shared memory, and ldmatrix reads either orientation; a warp's
@@ -48,10 +49,10 @@
 // key and value pad differently), shares of the measured copy rate in brackets:
 //   32 tokens x 16 lanes x 4 heads of 64/64: 12 and 15 us: one chunk's chain of
 //     loads, splits and products, mostly first fetches of instructions
-//   512 x 256 x 4 of 32/32: 121 (34%) and 325 us
-//   1024 x 64 x 8 of 64/64: 234 (36%) and 625 us; of 64/128: 416 and 1148 us
-//   2048 x 8 x 8 of 128/128: 172 and 530 us
-//   8191 x 2 x 8 of 64/64: 115 and 313 us, in segments
+//   512 x 256 x 4 of 32/32: 122 (34%) and 328 us
+//   1024 x 64 x 8 of 64/64: 240 (35%) and 637 us; of 64/128: 424 and 1086 us
+//   2048 x 8 x 8 of 128/128: 173 and 504 us
+//   8191 x 2 x 8 of 64/64: 118 and 319 us, in segments
 //
 // A product with a masked-out factor multiplies by zero, which infinities and
 // NaN survive. So a chunk whose results are not all finite is done again
@@ -136,15 +137,18 @@ __device__ __forceinline__ float2 join2(uint32_t hi, uint32_t lo) {
   return make_float2(h.x + l.x, h.y + l.y);
 }
 
-// The power of two that brings a largest magnitude to [2^14, 2^15), from
-// 2^-40 (beyond, halves overflow to infinity and the chunk is done token by
-// token) to 2^80: a tile whose largest value is below 2^-76 has fewer bits, and
-// what two such tiles make is below float's normal range.
+// The power of two that brings the state's largest magnitude
+// to [2^14, 2^15), from 2^-40 to 2^90. Beyond, at either end, the chunk is done
+// token by token (tile_fits).
+constexpr int kLaTileMost = 90;
 __device__ __forceinline__ float tile_scale(uint32_t max_bits) {
   if (max_bits == 0) return 1.f;
   int e = 141 - static_cast<int>(max_bits >> 23);
-  e = max(-40, min(80, e));
+  e = max(-40, min(kLaTileMost, e));
   return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
+}
+__device__ __forceinline__ bool tile_fits(uint32_t max_bits) {
+  return max_bits < 0x7f800000u && (max_bits == 0 || (max_bits >> 23) >= 141 - kLaTileMost);
 }
 // Of a power of two. Products of such inverses may run out of range to zero,
 // as what they scale does; a product of the powers themselves may not.
@@ -152,12 +156,17 @@ __device__ __forceinline__ float pow2_inverse(float s) {
   return __uint_as_float((254u << 23) - __float_as_uint(s));
 }
 
-// A row of k or v has a power of two of its own, that brings its largest value to
-// [2^14, 2^15): from 2^-40 to 2^62. No power (kLaNone) for a row of zeros.
-constexpr int kLaNone = -128, kLaLeast = -40, kLaMost = 62;
+// A row of q, k or v has a power of two of its own, that brings its largest value to
+// [2^14, 2^15): from 2^-40 to 2^100 (smaller rows: row_fits), those of a token's k
+// and v 2^124 at most. No power
+// (kLaNone) for a row of zeros.
+constexpr int kLaNone = -128, kLaLeast = -40, kLaMost = 100, kLaBoth = 124;
 __device__ __forceinline__ int row_exp(uint32_t max_bits) {
   if (max_bits == 0) return kLaNone;
   return max(kLaLeast, min(kLaMost, 141 - static_cast<int>(max_bits >> 23)));
+}
+__device__ __forceinline__ bool row_fits(uint32_t max_bits) {
+  return max_bits < 0x7f800000u && (max_bits == 0 || (max_bits >> 23) >= 141 - kLaMost);
 }
 __device__ __forceinline__ float pow2(int e) {  // -126 .. 127
   return __uint_as_float(static_cast<uint32_t>(127 + e) << 23);
@@ -168,9 +177,12 @@ __device__ __forceinline__ float pow2_above(float x) {
   return x == 0.f ? 1.f : pow2(max(-126, static_cast<int>(__float_as_uint(x) >> 23) - 126));
 }
 // A token's size, the inverse of what its k and v were scaled by, as the
-// exponent of a float (3 to 207; 0 where either is zero).
-__device__ __forceinline__ uint32_t token_size(int ek, int ev) {
-  return ek == kLaNone || ev == kLaNone ? 0u : static_cast<uint32_t>(127 - ek - ev);
+// exponent of a float (3 to 207; 0 where either is zero). `fine` becomes false
+// where the token is too small for one.
+__device__ __forceinline__ uint32_t token_size(int ek, int ev, bool& fine) {
+  if (ek == kLaNone || ev == kLaNone) return 0u;
+  fine &= ek + ev <= kLaBoth;
+  return static_cast<uint32_t>(127 - min(ek + ev, kLaBoth));
 }
 __device__ __forceinline__ float size_float(uint32_t size) { return __uint_as_float(size << 23); }
 // Tokens alike within 2^8: then the bound of a row's scores is the largest
@@ -323,7 +335,7 @@ __device__ __forceinline__ bool store_tile(uint32_t base, uint32_t part,
     for (int e = 0; e < 4; ++e) top = max(top, __float_as_uint(x[u][e]) & 0x7fffffffu);
     top = row_max<Q>(top);
     const int e = row_exp(top);
-    fine &= top < 0x7f800000u && (top == 0 || (top >> 23) >= 141 - kLaMost);
+    fine &= row_fits(top);
     lost += la_short(x[u], e);
     const float scale = row_scale(e);
     if (threadIdx.x % Q == 0) exps[r0 + u * (kLaThreads / Q)] = static_cast<int8_t>(e);
@@ -533,7 +545,7 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
         const int j = w * 32 + lane;
-        size[w] = token_size(kexp[j], kexp[kLaChunk + j]);
+        size[w] = token_size(kexp[j], kexp[kLaChunk + j], finite);
         high = max(high, size[w]);
         low = min(low, size[w] == 0 ? 255u : size[w]);
         zeros |= size[w] == 0 && j < len;
@@ -585,7 +597,7 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
       }
       if constexpr (OUT) {
         const uint32_t top = max(max(maxima[0], maxima[1]), max(maxima[2], maxima[3]));
-        finite &= top < 0x7f800000u;
+        finite &= tile_fits(top);
         sst = tile_scale(top);
         const int es = static_cast<int>(__float_as_uint(sst) >> 23) - 127;
         if (la_dwarfs(es, low)) {
@@ -672,8 +684,8 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
               top = max(top, __float_as_uint(x[k][(e >> 1) * 4 + half * 2 + (e & 1)]) & 0x7fffffffu);
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
           top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-          sq[half] = tile_scale(top);
-          finite &= top < 0x7f800000u;
+          sq[half] = row_scale(row_exp(top));
+          finite &= row_fits(top);
         }
         finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(a, len);
 #pragma unroll
@@ -1149,7 +1161,7 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
           for (int e = 0; e < 4; ++e) xk[u][e] *= a.kscale;
         const uint32_t top = row_max<DK / 4>(tc_max(xk[u]));
         ek[u] = row_exp(top);
-        finite &= top == 0 || (top >> 23) >= 141 - kLaMost;
+        finite &= row_fits(top);
         lost += la_short(xk[u], ek[u]);
         tc_put(sbase + T::kK0 + tc_slot<DK>() + u * RK * 128, T::kQ, xk[u], row_scale(ek[u]));
         if (T::kTwo && tid % (DK / 4) == 0)
@@ -1159,7 +1171,7 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
       for (int u = 0; u < NV; ++u) {
         const uint32_t top = row_max<16>(tc_max(xv[u]));
         const int ev = row_exp(top);
-        finite &= top == 0 || (top >> 23) >= 141 - kLaMost;
+        finite &= row_fits(top);
         lost += la_short(xv[u], ev);
         const float scale = row_scale(ev);
 #pragma unroll
@@ -1170,7 +1182,7 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
           if (T::kTwo)
             kexp[kTcChunk + r] = static_cast<int8_t>(ev);
           else
-            size[r] = static_cast<uint8_t>(token_size(ek[u % NK], ev));
+            size[r] = static_cast<uint8_t>(token_size(ek[u % NK], ev, finite));
         }
       }
     }
@@ -1183,9 +1195,10 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
         top = max(top, max(max(x.x, x.y), max(x.z, x.w)));
       }
       sst = tile_scale(top);
+      finite &= tile_fits(top);
     }
     if (T::kTwo && tid < kTcChunk)
-      size[tid] = static_cast<uint8_t>(token_size(kexp[tid], kexp[kTcChunk + tid]));
+      size[tid] = static_cast<uint8_t>(token_size(kexp[tid], kexp[kTcChunk + tid], finite));
     {
 #pragma unroll
       for (int m = 0; m < MS; ++m)
@@ -1210,7 +1223,9 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
       // two of 64.
 #pragma unroll
       for (int u = 0; u < NK; ++u) {
-        const float sq = tile_scale(row_max<DK / 4>(tc_max(xq[u])));
+        const uint32_t top = row_max<DK / 4>(tc_max(xq[u]));
+        const float sq = row_scale(row_exp(top));
+        finite &= row_fits(top);
         if (tid % (DK / 4) == 0)
           qexp[tid / (DK / 4) + u * RK] =
               static_cast<int8_t>(static_cast<int>(__float_as_uint(sq) >> 23) - 127);
@@ -1676,9 +1691,9 @@ static int la_pad_v(int vd) { return vd <= 32 ? 32 : 64; }
 // The scan that writes results takes the tcgen05 form where its tiles of 128
 // tokens and 64 columns are not mostly empty. Times of 64 lanes x 8 heads on
 // mma.sync and on tcgen05 in us:
-//   64 tokens, 64/64: 27, 32; 65: 39, 32; 128: 42, 38; 1024: 249, 190
-//   1024 tokens, key 64, value 32: 164, 186; 32/64: 160, 298; 128/32: 401, 308;
-//   2048 x 8 lanes, 128/128: 399, 152
+//   64 tokens, 64/64: 24, 33; 65: 39, 33; 128: 44, 36; 1024: 296, 236
+//   1024 tokens, key 64, value 32: 190, 226; 128/32: 460, 336;
+//   2048 x 8 lanes, 128/128: 426, 168
 static bool la_tc(const LaArgs& a) {
   return a.steps > 64 && (a.kd > 64 || (a.kd > 32 && a.vd > 32));
 }
