@@ -678,7 +678,7 @@ enum { TTRL_ACT_NONE = 0, TTRL_ACT_RELU = 1, TTRL_ACT_SILU = 2 };
 
 /* y = act(hat * weight + bias) over `images` blocks of [spatial][channels]
  * channels-last rows (the rows ttrl_conv_fprop writes; spatial = 1: one row
- * an image), hat = (x - mean) / sqrt(var + eps) with mean and (biased)
+ * an image; up to 65535 * 256 channels), hat = (x - mean) / sqrt(var + eps) with mean and (biased)
  * variance over the spatial * channels / groups elements of an image's group.
  * weight, bias: [channels], NULL for 1 and 0. stats ([images][groups][2]:
  * mean, 1 / sqrt(var + eps)) is what the backward reads; NULL: not written.

@@ -1,6 +1,7 @@
 """Group norm where its plans (a warp, a block, a cluster an image, passes over
 global memory) have to agree."""
 
+import ctypes
 import subprocess
 import sys
 
@@ -113,3 +114,18 @@ def test_results_do_not_depend_on_the_shapes_before():
         return run.stdout.strip().splitlines()[-1]
 
     assert first("narrow") == first("wide", "narrow")
+
+
+def test_more_channels_than_a_grid_holds_are_refused():
+    """By the extents alone: no pointer is looked at."""
+    from ttrl_b200._lib import lib
+    p, null = ctypes.c_void_p(64), None
+    for channels in (65535 * 256 + 1, 1 << 30):
+        assert lib().ttrl_group_norm_workspace_bytes(1, 1, channels, 1, 0) == 0
+        assert lib().ttrl_group_norm_fwd(p, null, null, p, null, 1, 1, channels, 1, 1e-5, 0, null,
+                                         0, null) != 0
+        assert b"channels" in lib().ttrl_last_error()
+        assert lib().ttrl_group_norm_bwd(p, p, null, null, p, p, null, null, 1, 1, channels, 1, 0,
+                                         0, 0, null, 0, null) != 0
+        assert b"channels" in lib().ttrl_last_error()
+    assert lib().ttrl_group_norm_workspace_bytes(1, 1, 65535 * 256, 1, 0) > 0

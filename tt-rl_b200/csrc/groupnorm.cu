@@ -1587,9 +1587,12 @@ static GnWs gn_ws(const GnPlan& p, long long images, int channels, int groups, b
   return w;
 }
 
+// The passes over global memory have a grid row for every 256 channels or quads.
+constexpr int kGnMaxChannels = 65535 * kGnWideThreads;
+
 static bool gn_shape_ok(int images, int spatial, int channels, int groups) {
   if (images <= 0 || spatial <= 0 || channels <= 0 || groups <= 0) return false;
-  if (channels % groups != 0) return false;
+  if (channels % groups != 0 || channels > kGnMaxChannels) return false;
   // Counts of rows and images step past their ends by less than 2^16.
   constexpr long long kMost = (1ll << 31) - (1ll << 16);
   return static_cast<long long>(spatial) * channels < kMost &&
@@ -1771,6 +1774,9 @@ static int gn_check(const char* what, int images, int spatial, int channels, int
                      groups);
   if (act != TTRL_ACT_NONE && act != TTRL_ACT_RELU && act != TTRL_ACT_SILU)
     return set_error(TTRL_EINVAL, "%s: unknown activation %d", what, act);
+  if (channels > kGnMaxChannels)
+    return set_error(TTRL_EUNSUPPORTED, "%s: %d channels, up to %d are served", what, channels,
+                     kGnMaxChannels);
   if (images > 0 && !gn_shape_ok(images, spatial, channels, groups))
     return set_error(TTRL_EUNSUPPORTED, "%s: an image of more than 2^31 - 2^16 elements, or as many groups in all",
                      what);
