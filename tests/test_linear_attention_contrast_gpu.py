@@ -16,8 +16,9 @@ from tests.test_linear_attention_gpu import plain  # noqa: E402
 gpu = pytest.mark.gpu
 TOL = 2e-6
 
-#: steps, lanes, heads, key, value: one chunk, several on either kernel, segments
-SHAPES = [(50, 3, 2, 64, 64), (150, 2, 2, 32, 32), (200, 2, 2, 64, 64), (200, 2, 3, 100, 90),
+#: steps, lanes, heads, key, value: a few tokens, one chunk, several on either
+#: kernel, segments
+SHAPES = [(6, 3, 2, 64, 64), (9, 2, 2, 128, 33), (50, 3, 2, 64, 64), (150, 2, 2, 32, 32), (200, 2, 2, 64, 64), (200, 2, 3, 100, 90),
           (1500, 1, 2, 64, 64)]
 
 

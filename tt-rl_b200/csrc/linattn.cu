@@ -231,8 +231,8 @@ __device__ __forceinline__ bool la_dwarfs(int es, uint32_t least_size) {
   return es + static_cast<int>(least_size) + 30 < 127;
 }
 __device__ __forceinline__ int la_rows(int len) { return len >= 64 ? 2 : 1; }
-__device__ __forceinline__ int la_spare(const LaArgs& a, int len) {
-  return len >= 64 ? 2 : 1 + min(3, (len * (a.kd + a.vd)) >> 11);
+__device__ __forceinline__ int la_spare(int len) {
+  return len >= 64 ? 2 : max(1, min(4, len / 2));
 }
 
 // Scores of two such tiles are below 128 * 2^30: times this, a half.
@@ -687,7 +687,7 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
           sq[half] = row_scale(row_exp(top));
           finite &= row_fits(top);
         }
-        finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(a, len);
+        finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(len);
 #pragma unroll
         for (int k = 0; k < NK; ++k)
 #pragma unroll
@@ -807,7 +807,7 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
         }
       }
     } else {
-      finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(a, len);
+      finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(len);
     }
     // The state behind the chunk: this chunk's sum on its own, then one fp32
     // multiply and add.
@@ -897,11 +897,10 @@ __global__ void __launch_bounds__(kLaThreads, DK <= 64 ? 4 : DV == 64 ? 2 : 3)
 // both orientations: k is read token by token for the scores and transposed
 // for the state.
 //
-// Bound: the chain of a chunk. Alone on an SM a block takes about 20,000 cycles
-// for one, of which the products are 6,000, loads 5,000 and splits and
-// exchanges the rest; two blocks an SM (keys of 64: 112 KB each) fill each
-// other's waits, 12,000 a chunk, at 48% of the issue slots and 35% of the
-// tensor pipe; memory alone would allow 5,600. Keys of 128 leave room for one
+// Bound: the chain of a chunk: loads, scales and splits, the products (6,000
+// cycles), weights and output. Two blocks an SM (keys of 64: 113 KB each) fill
+// each other's waits, 16,000 cycles a chunk, at 49% of the issue slots and 24% of
+// the tensor pipe; memory alone would allow 5,600. Keys of 128 leave room for one
 // block, of 512 threads (256: 11% slower). Tried and not kept: k copied ahead
 // to shared memory (the same at 64, 12% slower at 128), k ahead in registers
 // (spills at 64, 2% at 128), v's and the state's splits behind the first
@@ -1234,7 +1233,7 @@ __global__ void __launch_bounds__(LaTc<DK>::kThreads, DK == 64 ? 2 : 1)
     }
     fence_proxy_async_smem();
     tc_fence_before();
-    finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(a, len);
+    finite &= __syncthreads_count(lost >= la_rows(len)) < la_spare(len);
     if (tid == 0 && !dead) {
       tc_fence_after();
       const uint64_t qd = umma_desc(sbase + T::kQ0, 16, 1024, kLayoutSw128);
