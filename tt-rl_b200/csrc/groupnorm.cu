@@ -25,8 +25,8 @@
 //    block, so its weights, group indices and column sums are registers too.
 //    4096 x 49 x 64: 31 us (51%), 43 us (55%);
 //  - longer: one thread-block cluster an image, its rows staged in shared
-//    memory forward, read again from L2 backward. 512 x 1764 x 90: 173 us
-//    (58%), 340 us (45%): 25 to 30 warps an SM with one barrier of the cluster
+//    memory forward, read again from L2 backward. 512 x 1764 x 90: 176 us
+//    (57%), 341 us (44%): 25 to 30 warps an SM with one barrier of the cluster
 //    an image do not cover the loads, the group sums (3000 cycles an image) and
 //    the exchange (2500). Tried: the next image's rows fetched while this one
 //    is written (the same); images dealt out as clusters finish, by a counter
@@ -39,8 +39,11 @@
 // passes over global memory with per-column partial sums: 21 images of 5879 x
 // 128 46 us and 71 us. (Batches of images whose sums one launch takes while it
 // writes the batch before were 1.2 to 1.7 times slower: the sums' tail.)
-// Variance is taken about means (merged by the pairwise update of count, mean
-// and sum of squares), never as the difference of two large sums. Every sum
+// Variance is taken about means within a thread and in the passes over global
+// memory (merged by the pairwise update of count, mean and sum of squares). The
+// threads of a block or cluster add sums and sums of squares in 64 bits and
+// subtract there: a mean of 10^k deviations costs 2k of 15 digits, fewer than its
+// values' own roundings to float have cost. Every sum
 // has a fixed order: results are bit for bit the same from run to run.
 #include <algorithm>
 #include <cstring>
